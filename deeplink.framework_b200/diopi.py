@@ -177,6 +177,9 @@ SIGNATURES = {
     "diopiMultinomial": "TtibG", "diopiIndexPutInp": "TtLb",
     # additions of this library (include/diopi/functions_b200.h): fused steps of a decode iteration
     "diopiB200MmSwiGLU": "TTT", "diopiB200AddRMSNorm": "TTTTtd", "diopiB200RopeAppendKV": "TTTTTTi",
+    # and the int8 key / value cache with the attention over it
+    "diopiB200RopeQuantAppendKV": "tTttTTTTTb", "diopiB200DequantKV": "TTTTTTt",
+    "diopiB200CachedAttention": "TtTTtTtTd", "diopiB200SharedPrefixAttention": "TtTTTTtTtTd",
 }
 
 _CTYPES = {"T": ctypes.c_void_p, "t": ctypes.c_void_p, "s": ctypes.POINTER(_Scalar), "i": ctypes.c_int64, "d": ctypes.c_double,

@@ -145,6 +145,20 @@ class TpGroup:
         self.comm = None
 
 
+class QuantKVCache:
+    """One layer's keys and values as int8 codes with a float32 scale per row: 132 bytes a row of 128 values instead of 256. Layout and
+    rounding are the library's (include/diopi/functions_b200.h); `args` is what its calls take."""
+
+    def __init__(self, batch, kv_heads, capacity, head_dim, device="cuda:0"):
+        self.batch, self.kv_heads, self.capacity, self.head_dim = batch, kv_heads, capacity, head_dim
+        self.k, self.v = (torch.zeros((batch, kv_heads, capacity, head_dim), dtype=torch.int8, device=device) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.zeros((batch, kv_heads, capacity), dtype=torch.float32, device=device) for _ in range(2))
+
+    @property
+    def args(self):
+        return self.k, self.k_scale, self.v, self.v_scale
+
+
 class DecoderLayer:
     def __init__(self, cfg, weights, dtype=torch.bfloat16, device="cuda:0", tp_rank=0, tp_size=1, tp_group=None):
         self.hidden = cfg.hidden
@@ -489,3 +503,113 @@ class DecoderLayer:
         out = self._ffn(ctx, h)
         ctx.release_workspace()
         return out
+
+    # ---- int8 cache, ragged batches, shared prompts ------------------------------------------------------------------
+    # A prompt that the whole batch shares is passed as `prefix`: its rotated keys and its values, [P, local kv heads, D] in the
+    # model's type (one sequence's prefill gives them, prefix_kv). The sequences' own slots then stand for positions P, P + 1, ...
+    def _cached_tables(self, cache, prefix):
+        first = 0 if prefix is None else prefix[0].shape[0]
+        return self._tables_for(("cached", first, cache.capacity), torch.arange(first, first + cache.capacity))
+
+    def _cached_supported(self):
+        assert self.dtype in (torch.bfloat16, torch.float16) and self.head_dim in (64, 128), "the int8 cache serves bfloat16 / float16 and head dim 64 or 128"
+
+    def prefix_kv(self, x, ctx=None):
+        """Rotated keys and values of a shared prompt, from the layer's input x [P, hidden] for it."""
+        ctx = ctx or diopi.Context()
+        n, d, hk = x.shape[0], self.head_dim, self.kv_heads
+        hn = self._like(x)
+        self._call(diopi.diopiRMSNorm, ctx, hn, None, x, [self.hidden], self.attention_norm, None, self.eps)
+        k, v = self._linear(ctx, hn, self.wk).view(n, hk, d), self._linear(ctx, hn, self.wv).view(n, hk, d)
+        cos, sin = self._tables_for(("prefill", n), torch.arange(n))
+        return self._rope(ctx, k, cos, sin), v
+
+    def prefill_cached(self, x, batch, seq, cache, start=0, prefix=None, ctx=None):
+        """A chunk of `seq` tokens per sequence, x [batch * seq, hidden], into slots start .. start + seq - 1 of a QuantKVCache whose
+        earlier slots are filled. The chunk attends to what the cache holds, itself included, as a later decode step will see it:
+        the rows are read back and go through the fused attention (head dim 128)."""
+        ctx = ctx or diopi.Context()
+        self._cached_supported()
+        assert self.head_dim == 128, "the fused prefill attention has head dim 128"
+        assert 0 <= start and start + seq <= cache.capacity, "slots %d .. %d of a cache of %d" % (start, start + seq - 1, cache.capacity)
+        d, hq, hk, length = self.head_dim, self.heads, self.kv_heads, start + seq
+        wqkv, _ = self._merged_weights()
+        hn = self._like(x)
+        self._call(diopi.diopiRMSNorm, ctx, hn, None, x, [self.hidden], self.attention_norm, None, self.eps)
+        qkv = self._linear(ctx, hn, wqkv).view(batch, seq, (hq + 2 * hk) * d)
+        cos, sin = self._cached_tables(cache, prefix)
+        positions = self._empty(batch, dtype=torch.int64)
+        self._call(diopi.diopiFill, ctx, positions, start)
+        q = self._empty(batch, seq, hq, d)
+        self._call(diopi.diopiB200RopeQuantAppendKV, ctx, q, qkv, cos, sin, positions, *cache.args, self.interleaved)
+        shared = 0 if prefix is None else prefix[0].shape[0]
+        keys, vals = self._empty(batch, shared + length, hk, d), self._empty(batch, shared + length, hk, d)
+        if shared:
+            for rows, one in ((keys, prefix[0]), (vals, prefix[1])):
+                self._call(diopi.diopiCopyInp, ctx, one.unsqueeze(0).expand(batch, shared, hk, d), rows[:, :shared])
+        self._call(diopi.diopiB200DequantKV, ctx, keys[:, shared:], vals[:, shared:], *cache.args, None)
+        merged = self._empty(batch, seq, hq, d)
+        self._call(diopi.diopiMultiHeadAttention, ctx, q, keys, vals, 0.0, True, False, 1.0 / math.sqrt(d), merged, None, None, None)
+        attn = self._linear(ctx, merged.view(batch * seq, hq * d), self.wo)
+        self._all_reduce(ctx, attn)
+        h = self._like(x)
+        self._call(diopi.diopiAdd, ctx, h, x, attn, 1)
+        out = self._ffn(ctx, h)
+        ctx.release_workspace()
+        return out
+
+    def decode_cached(self, x, cache, positions, lengths, prefix=None, ctx=None):
+        """One token per sequence, x [batch, hidden], at each sequence's own place: positions int64 [batch] (the slot that receives the
+        new key and value; negative: the sequence is idle), lengths int64 [batch] (positions + 1; 0 for idle ones)."""
+        ctx = ctx or diopi.Context()
+        self._cached_supported()
+        b, d, hq, hk = x.shape[0], self.head_dim, self.heads, self.kv_heads
+        wqkv, w13 = self._merged_weights()
+        hn = self._like(x)
+        self._call(diopi.diopiRMSNorm, ctx, hn, None, x, [self.hidden], self.attention_norm, None, self.eps)
+        qkv = self._linear(ctx, hn, wqkv)
+        cos, sin = self._cached_tables(cache, prefix)
+        q, av = self._empty(b, hq, d), self._empty(b, hq, d)
+        self._call(diopi.diopiB200RopeQuantAppendKV, ctx, q, qkv, cos, sin, positions, *cache.args, self.interleaved)
+        if prefix is None:
+            self._call(diopi.diopiB200CachedAttention, ctx, av, None, q, *cache.args, lengths, 1.0 / math.sqrt(d))
+        else:
+            self._call(diopi.diopiB200SharedPrefixAttention, ctx, av, None, q, prefix[0], prefix[1], *cache.args, lengths, 1.0 / math.sqrt(d))
+        attn = self._linear(ctx, av.view(b, hq * d), self.wo)
+        self._all_reduce(ctx, attn)
+        if b <= 128:   # the rows diopiB200MmSwiGLU serves
+            h, hn2 = self._like(x), self._like(x)
+            self._call(diopi.diopiB200AddRMSNorm, ctx, h, hn2, x, attn, self.ffn_norm, self.eps)
+            g = self._empty(b, self.ffn)
+            self._call(diopi.diopiB200MmSwiGLU, ctx, g, hn2, w13.t())
+            out = self._like(x)
+            if self.tp_rank == 0:
+                self._call(diopi.diopiAddmm, ctx, out, h, g, self.w2.t(), 1.0, 1.0)
+            else:
+                self._call(diopi.diopiMm, ctx, out, g, self.w2.t())
+            self._all_reduce(ctx, out)
+        else:
+            h = self._like(x)
+            self._call(diopi.diopiAdd, ctx, h, x, attn, 1)
+            out = self._ffn(ctx, h)
+        if self._keep is None:   # a graph keeps the workspace it was captured with
+            ctx.release_workspace()
+        return out
+
+    def capture_decode_cached(self, x, cache, positions, lengths, prefix=None, stream=None):
+        """Captures decode_cached into a CUDA graph, like capture_decode: (replay, out). The graph follows x, positions and lengths
+        when they change in place, so one graph serves every step. It owns its context: the workspace the capture took stays its
+        own for as long as `replay` lives. The step must have run once before."""
+        ctx = diopi.Context(stream=stream)
+        self._keep = [x, cache, positions, lengths, prefix, ctx]
+        devapis.graphBeginCapture(ctx.stream)
+        try:
+            out = self.decode_cached(x, cache, positions, lengths, prefix, ctx)
+        finally:
+            graph = devapis.graphEndCapture(ctx.stream)
+            keep, self._keep = self._keep, None
+
+        def replay(_keep=keep):
+            devapis.graphLaunch(graph, ctx.stream)
+        replay.graph = graph
+        return replay, out

@@ -89,6 +89,53 @@ DIOPI_API diopiError_t diopiB200RopeAppendKV(diopiContextHandle_t ctx, diopiTens
                                              diopiConstTensorHandle_t cos, diopiConstTensorHandle_t sin, diopiTensorHandle_t k_cache,
                                              diopiTensorHandle_t v_cache, int64_t position);
 
+/* A key / value cache in int8, and decode attention over caches of ragged lengths. No counterparts in the reference, whose cache
+ * is in the model's type with one position for the whole batch (dicp/test/model/llama/model.py:134-138) and whose decode attention
+ * walks the sequences one by one (dicp/dicp/vendor/AscendGraph/ext_ops.py:89-126).
+ *
+ * Cache: codes int8 [B, Hkv, L, D] and scales float32 [B, Hkv, L], one scale per row; a row stands for code * scale. D is 64 or
+ * 128. Codes may have any pitches that are multiples of 16 with contiguous rows (16-byte aligned), scales any pitches with
+ * neighbouring slots next to each other. positions / lengths are int64 [B] in device memory: one launch serves sequences at
+ * different places, and a captured graph follows them when they change. bfloat16 / float16 everywhere else.
+ *
+ * diopiB200RopeQuantAppendKV  qkv [B, S, (Hq + 2 Hkv) D], the output of ONE projection for S tokens of every sequence (or
+ *                      [B, (Hq + 2 Hkv) D] for one token): q rotated -> q_out [B, S, Hq, D] ([B, Hq, D]); k rotated, v -> codes and
+ *                      scales of the slots positions[b] + s. scale = max|y| / 127, code = y * (127 / max|y|) to the nearest (ties
+ *                      to even), formed from the fp32 rotation, which is not rounded in between; a row of zeros has scale 0, a
+ *                      row that holds an infinity or a NaN gets scale NaN and reads back as NaN. cos / sin: dense float32
+ *                      [rows, R / 2] tables indexed by position; the first R (a multiple of 8, at most D) values of a head turn,
+ *                      in pairs (i, i + R / 2) or, `interleaved`, (2i, 2i + 1), the others stay; a long-context scaling of the
+ *                      angles is the table's content. Both NULL: nothing is rotated. q_out NULL: qkv holds k and v only.
+ *                      A sequence with a negative position is idle: nothing is written for it. Tokens whose slot lies behind
+ *                      the cache or behind the tables are skipped the same way. Every other slot keeps its content.
+ * diopiB200DequantKV   k_out / v_out [B, S, Hkv, D] = code * scale of the slots positions[b] + s (NULL: 0 + s), rounded once.
+ *                      Tokens without such a slot (negative position, behind the cache) keep what k_out / v_out held.
+ * diopiB200CachedAttention  out [B, Hq, D] = softmax(scale * q K^T) V over the first lengths[b] slots (clamped to [0, L]) of sequence
+ *                      b's cache; Hq / Hkv query heads share a key head. k_scale / v_scale NULL: k_cache / v_cache
+ *                      hold q's dtype (pitches multiples of 8 elements). An empty sequence gives zeros and a
+ *                      softmax_lse of -inf. softmax_lse: optional float32 [B, Hq], the log of the softmax denominator.
+ * diopiB200SharedPrefixAttention  the same over the rows of a prompt that all sequences share, prefix_k / prefix_v [P, Hkv, D] in q's
+ *                      dtype (any positive pitches that are multiples of 8), followed by the sequence's own lengths[b] slots. The
+ *                      prompt is stored once and read once for the batch.
+ * out must not overlap an input. The attention calls take workspace through diopiRequireBuffer; a graph that captured one needs
+ * that workspace for its replays, so its context keeps it (no release, no other use of the context) while the graph lives. */
+DIOPI_API diopiError_t diopiB200RopeQuantAppendKV(diopiContextHandle_t ctx, diopiTensorHandle_t q_out, diopiConstTensorHandle_t qkv,
+                                                  diopiConstTensorHandle_t cos, diopiConstTensorHandle_t sin, diopiConstTensorHandle_t positions,
+                                                  diopiTensorHandle_t k_cache, diopiTensorHandle_t k_scale, diopiTensorHandle_t v_cache,
+                                                  diopiTensorHandle_t v_scale, bool interleaved);
+DIOPI_API diopiError_t diopiB200DequantKV(diopiContextHandle_t ctx, diopiTensorHandle_t k_out, diopiTensorHandle_t v_out,
+                                          diopiConstTensorHandle_t k_cache, diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v_cache,
+                                          diopiConstTensorHandle_t v_scale, diopiConstTensorHandle_t positions);
+DIOPI_API diopiError_t diopiB200CachedAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiTensorHandle_t softmax_lse,
+                                                diopiConstTensorHandle_t q, diopiConstTensorHandle_t k_cache, diopiConstTensorHandle_t k_scale,
+                                                diopiConstTensorHandle_t v_cache, diopiConstTensorHandle_t v_scale,
+                                                diopiConstTensorHandle_t lengths, double scale);
+DIOPI_API diopiError_t diopiB200SharedPrefixAttention(diopiContextHandle_t ctx, diopiTensorHandle_t out, diopiTensorHandle_t softmax_lse,
+                                                      diopiConstTensorHandle_t q, diopiConstTensorHandle_t prefix_k,
+                                                      diopiConstTensorHandle_t prefix_v, diopiConstTensorHandle_t k_cache,
+                                                      diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v_cache,
+                                                      diopiConstTensorHandle_t v_scale, diopiConstTensorHandle_t lengths, double scale);
+
 #ifdef __cplusplus
 }
 #endif
