@@ -5,7 +5,7 @@
 //   diopiB200DequantKV          codes * scales of a window of slots, back in the model's type
 //
 // A row y (D values, fp32; k after the rotation, which is not rounded in between) is stored as
-//   scale = max|y| / 127,   code = rint(y * (127 / max|y|)) in [-127, 127],   so |y - code * scale| <= 0.5 scale.
+//   scale = max|y| / 127,   code = rint(y / scale) in [-127, 127],   so |y - code * scale| <= 0.5 scale.
 // A row of zeros has scale 0 and codes 0; a row that holds an infinity or a NaN has scale NaN, so that it reads back as NaN
 // rather than as finite numbers. Symmetric codes need no offset, and one scale per row factors out of q . k and of p * v.
 #include "copy.h"
@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(256) rope_quant_append_kernel(const AppendPara
     const int c = threadIdx.x % LANES;
     const int heads = p.Hq + 2 * p.Hkv;
     const bool live = item < p.items;
+    grid_launch_dependents();   // the attention that follows may set itself up meanwhile
     const int64_t token = live ? item / heads : 0;
     const int h = live ? static_cast<int>(item - token * heads) : 0;
     const int64_t b = token / p.S, s = token - b * p.S;
@@ -99,12 +100,20 @@ __global__ void __launch_bounds__(256) rope_quant_append_kernel(const AppendPara
     const float scale = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
     uint32_t code[8];
     if (amax > 1e-30f && finite) {
-        // y * (127 / max|y|) + 1.5 * 2^23, rounded once to nearest even: the low byte of the sum is the code
+        // y * (127 / max|y|) + 1.5 * 2^23, rounded once to nearest even: the low byte of the sum is the code. Where the product is
+        // within 2^-12 of a tie the quotient itself decides (the product is within 127 * 2^-22 of it): a row's values are few
+        // bits long, so half of the largest one, code 63.5, is no rare value.
         const float r = 127.f / amax;
+        float off = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            code[2 * i] = __float_as_uint(fmaf(y[i].x, r, 12582912.f));
-            code[2 * i + 1] = __float_as_uint(fmaf(y[i].y, r, 12582912.f));
+        for (int i = 0; i < 8; ++i) {
+            const float x = (i & 1) ? y[i >> 1].y : y[i >> 1].x, s = fmaf(x, r, 12582912.f);
+            code[i] = __float_as_uint(s);
+            off = fmaxf(off, fabsf(fmaf(x, r, 12582912.f - s)));
+        }
+        if (off > 0.5f - 0x1p-12f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) code[i] = static_cast<uint32_t>(__float2int_rn(((i & 1) ? y[i >> 1].y : y[i >> 1].x) / scale));
         }
     } else {
         // rows so small that 127 / max|y| may overflow, rows of zeros (also those whose scale underflows to zero), rows that are not finite

@@ -100,8 +100,8 @@ DIOPI_API diopiError_t diopiB200RopeAppendKV(diopiContextHandle_t ctx, diopiTens
  *
  * diopiB200RopeQuantAppendKV  qkv [B, S, (Hq + 2 Hkv) D], the output of ONE projection for S tokens of every sequence (or
  *                      [B, (Hq + 2 Hkv) D] for one token): q rotated -> q_out [B, S, Hq, D] ([B, Hq, D]); k rotated, v -> codes and
- *                      scales of the slots positions[b] + s. scale = max|y| / 127, code = y * (127 / max|y|) to the nearest (ties
- *                      to even), formed from the fp32 rotation, which is not rounded in between; a row of zeros has scale 0, a
+ *                      scales of the slots positions[b] + s. scale = max|y| / 127, code = y / scale to the nearest (ties to
+ *                      even), formed from the fp32 rotation, which is not rounded in between; a row of zeros has scale 0, a
  *                      row that holds an infinity or a NaN gets scale NaN and reads back as NaN. cos / sin: dense float32
  *                      [rows, R / 2] tables indexed by position; the first R (a multiple of 8, at most D) values of a head turn,
  *                      in pairs (i, i + R / 2) or, `interleaved`, (2i, 2i + 1), the others stay; a long-context scaling of the
