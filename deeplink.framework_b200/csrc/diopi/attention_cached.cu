@@ -570,25 +570,10 @@ __global__ void __launch_bounds__(128) cached_attention_join_kernel(const Cached
     if (threadIdx.x == 0 && p.lse != nullptr) p.lse[b * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh] = ll == 0.f ? -INFINITY : (base + log2f(ll)) * 0.6931471805599453f;
 }
 
-// A launch that may set itself up while the kernel before it in the stream ends (both kernels wait for it before they read).
-template <typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Args...), unsigned grid, unsigned threads, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename T, bool QUANT, int D>
 cudaError_t launch_own(const CachedAttnParams& p, int nt, cudaStream_t stream) {
-    return nt == 1 ? launch_dependent(cached_attention_kernel<T, QUANT, D, 1>, p.max_ctas, 128, stream, p)
-                   : launch_dependent(cached_attention_kernel<T, QUANT, D, 2>, p.max_ctas, 128, stream, p);
+    return nt == 1 ? launch_dependent(cached_attention_kernel<T, QUANT, D, 1>, static_cast<unsigned>(p.max_ctas), 128, 0, stream, p)
+                   : launch_dependent(cached_attention_kernel<T, QUANT, D, 2>, static_cast<unsigned>(p.max_ctas), 128, 0, stream, p);
 }
 template <typename T, int D>
 cudaError_t launch_attention(const CachedAttnParams& p, int nt, cudaStream_t stream) {
@@ -597,7 +582,7 @@ cudaError_t launch_attention(const CachedAttnParams& p, int nt, cudaStream_t str
         if (e != cudaSuccess) return e;
     }
     if (p.whole && p.own && p.prefix.splits == 0) return cudaSuccess;
-    return launch_dependent(cached_attention_join_kernel<T, D>, static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hq), 128, stream, p, 8 * nt);
+    return launch_dependent(cached_attention_join_kernel<T, D>, static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hq), 128, 0, stream, p, 8 * nt);
 }
 
 // CTAs of a variant that an SM holds at once.
@@ -670,6 +655,11 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
         B200_CHECK(vpk.aligned(16) && vpv.aligned(16) && kv_rows_fit(vpk, 8, true) && kv_rows_fit(vpv, 8, true),
                    "%s: prefix rows must be contiguous, 16-byte aligned, with positive pitches that are multiples of 8", name);
         P = vpk.shape[0];
+        for (const TensorView* x : {&vpk, &vpv}) {
+            const int64_t lo = x->stride[0] < x->stride[1] ? x->stride[0] : x->stride[1], hi = x->stride[0] < x->stride[1] ? x->stride[1] : x->stride[0];
+            B200_CHECK(P <= 1 || Hkv == 1 || hi % lo == 0, "%s: one of the prefix's pitches must be a multiple of the other", name);
+            B200_CHECK(hi < (1ll << 38), "%s: the prefix's pitches are too large", name);
+        }
     }
     B200_CHECK(P < (1ll << 30) && L < (1ll << 30), "%s: sequence too long", name);
     B200_CHECK(B < (1 << 24) && Hq < 65536 && B * Hq < 0x7fffffffLL, "%s: too many sequences or heads", name);

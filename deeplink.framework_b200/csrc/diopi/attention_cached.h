@@ -17,6 +17,23 @@ struct PrefixParts {
     int splits = 0;
 };
 
+// A launch that may set itself up while the kernel before it in the stream ends; the kernel waits (grid_dependency_wait) before it
+// touches global memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // q [B, Hq, D], k / v [P, Hkv, D], P > 0, checked by the caller. The pieces lie in workspace of `ctx`.
 diopiError_t prefix_attention(const char* name, diopiContextHandle_t ctx, const TensorView& q, const TensorView& k, const TensorView& v, float scale_log2,
                               PrefixParts* parts, cudaStream_t stream);

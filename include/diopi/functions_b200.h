@@ -115,7 +115,7 @@ DIOPI_API diopiError_t diopiB200RopeAppendKV(diopiContextHandle_t ctx, diopiTens
  *                      hold q's dtype (pitches multiples of 8 elements). An empty sequence gives zeros and a
  *                      softmax_lse of -inf. softmax_lse: optional float32 [B, Hq], the log of the softmax denominator.
  * diopiB200SharedPrefixAttention  the same over the rows of a prompt that all sequences share, prefix_k / prefix_v [P, Hkv, D] in q's
- *                      dtype (any positive pitches that are multiples of 8), followed by the sequence's own lengths[b] slots. The
+ *                      dtype (positive pitches that are multiples of 8, one a multiple of the other), followed by the sequence's own lengths[b] slots. The
  *                      prompt is stored once and read once for the batch.
  * out must not overlap an input. The attention calls take workspace through diopiRequireBuffer; a graph that captured one needs
  * that workspace for its replays, so its context keeps it (no release, no other use of the context) while the graph lives. */

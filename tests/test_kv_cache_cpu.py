@@ -180,6 +180,7 @@ def test_attention_over_the_models_type_refuses(on_device, change, match):
     ({"prefix_k": _aligned((P, 1, D), BF).expand(P, HKV, D)}, "pitches"),
     ({"prefix_k": _aligned((P, HKV, 2 * D), BF)[..., ::2]}, "contiguous"),
     ({"prefix_v": _host(_aligned((P, HKV, D), BF))}, "device"),
+    ({"prefix_v": _aligned((P * HKV * 3 * D,), BF).as_strided((P, HKV, D), (2 * D + 24, D, 1))}, "multiple of the other"),
 ])
 def test_prefix_refuses(on_device, change, match):
     _refused(on_device, "diopiB200SharedPrefixAttention", {**_prefix_args(), **change}, match)
