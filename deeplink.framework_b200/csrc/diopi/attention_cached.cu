@@ -18,20 +18,25 @@
 // index is free. For S^T a lane takes 16-byte chunks of its two key rows and the queries are laid out the same way; for O^T a lane
 // takes 16 neighbouring columns of its four key rows and pairs of keys are zipped with byte permutes. int8 codes become fp16 exactly
 // (a byte under the exponent of 1024, minus 1152), 1.25 instructions a value against 2 for a conversion to fp32 and its product.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
 #include "attention_cached.h"
 #include "device_utils.cuh"
 #include "diopi/functions_b200.h"
+#include "gemm.h"
 #include "kv_cache.h"
 
 namespace b200 {
 namespace {
 
 constexpr int kUnit = 64;            // keys per unit: 16 for each of a CTA's four warps
-constexpr int kMinUnits = 2;         // fewer units than this per CTA are not worth a piece of their own
+constexpr int kStart = 2;            // what a segment's start and end cost, in units (loading its queries, joining four warps, storing)
+constexpr int kMinPlaces = kStart + 1;   // fewer places than this per CTA are not worth a piece of their own
 constexpr int64_t kWholeKeys = 256;  // caches of at most this capacity: whole segments, one launch
+constexpr int64_t kWarpRows = 1024;  // from so many (sequence, query head) pairs on, the join has a warp for each instead of a CTA
+constexpr float kLowest = -3e38f;    // a running maximum before the first score: finite, so that no difference with it is NaN
 constexpr float kGrow = 8.f;         // the running maximum follows only when a score outgrows it by this (log2): P stays below 2^8
 
 struct CachedAttnParams {
@@ -53,7 +58,7 @@ struct CachedAttnParams {
     int max_ctas;
     float scale_log2;
     // workspace
-    int64_t* before;               // [B + 1]: units of the sequences before b (per key head and tile); [B]: of all
+    int* before;                   // [B + 1]: places of the sequences before b (per key head and tile); [B]: of all
     float* part_o;                 // [2 max_ctas (+ B Hkv tiles with a prefix)][8 NT][D]
     float2* part_ml;               // the same slots' running maximum (log2) and sum
     PrefixParts prefix;            // splits = 0: no prefix
@@ -65,20 +70,21 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-__device__ __forceinline__ int64_t units_of(const CachedAttnParams& p, int64_t b, int64_t* len) {
-    const int64_t n = min(max(p.lengths[b], int64_t(0)), p.L);
+// Units of sequence b and its length. An empty sequence counts one: someone has to write its zeros.
+__device__ __forceinline__ int units_of(const CachedAttnParams& p, int b, int* len) {
+    const int n = static_cast<int>(min(max(p.lengths[b], int64_t(0)), p.L));
     *len = n;
-    return n == 0 ? 1 : (n + kUnit - 1) / kUnit;   // an empty sequence is visited too: someone has to write its zeros
+    return max(1, (n + kUnit - 1) / kUnit);
 }
-// CTAs that get work, and the CTA that holds unit u of `total` dealt to `ctas`.
-__device__ __forceinline__ int64_t ctas_of(const CachedAttnParams& p, int64_t total) {
-    return min(static_cast<int64_t>(p.max_ctas), p.whole ? total : (total + kMinUnits - 1) / kMinUnits);
-}
-__device__ __forceinline__ int64_t holder(int64_t u, int64_t total, int64_t ctas) { return ((u + 1) * ctas - 1) / total; }
+// The dealing works on places: a segment takes kStart places, for what its start and end cost, and then one for each of its units.
+// Of `total` places dealt to `ctas` CTAs, CTA c has [total c / ctas, total (c + 1) / ctas); holder() is the CTA of a place.
+__device__ __forceinline__ int ctas_of(const CachedAttnParams& p, int total) { return min(p.max_ctas, (total + kMinPlaces - 1) / kMinPlaces); }
+__device__ __forceinline__ int place_of(int total, int c, int ctas) { return static_cast<int>(static_cast<int64_t>(total) * c / ctas); }
+__device__ __forceinline__ int holder(int place, int total, int ctas) { return static_cast<int>(((static_cast<int64_t>(place) + 1) * ctas - 1) / total); }
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, bf16>::value) {
+    if constexpr (std::is_same<T, bf16>::value) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -86,6 +92,19 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+// The same with a zero addend.
+template <typename T>
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, bf16>::value) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
     }
 }
 // Transposes an 8 x 8 matrix of 2-byte elements held as lane (row lane / 4, columns 2 (lane % 4), + 1).
@@ -101,135 +120,268 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t u) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint4 ldg16_once(const void* p) {
-    uint4 r;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ uint2 ldg8_once(const void* p) {
-    uint2 r;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-    return r;
-}
+// Shared memory of a variant: every warp's ring of key tiles (with the scales of the key and value rows) and value tiles, then the
+// two slots of the join.
+template <bool QUANT, int D, int NT>
+struct Ring {
+    static constexpr int kRow = D * (QUANT ? 1 : 2);                       // bytes of a cache row
+    static constexpr int kKeys = 16 * kRow + (QUANT ? 128 : 0);
+    static constexpr int kStage = kKeys + 16 * kRow;
+    static constexpr int kStages = QUANT || D == 64 ? 3 : 2;
+    static constexpr int kJoinFloats = NT * (D / 4 + 4) + 4;               // per lane: O, maximum and sum, reference
+    static constexpr int kWarp = kStages * kStage;
+    static constexpr int kTotal = 4 * kWarp + 2 * kJoinFloats * 128;
+    static constexpr int kCtas = std::min(3, 232448 / (kTotal + 1024 + 64));   // an SM holds
+};
+
+// Where a chunk of 16 bytes of a row lies, so that neither the copies nor the operand reads (eight lanes at a time: two key rows x
+// four chunks; four value rows x two chunks) meet in a bank.
+template <int CH>
+__device__ __forceinline__ int k_chunk(int row, int chunk) { return CH >= 8 ? chunk ^ ((row & 1) << 2) : chunk; }
+template <int CH>
+__device__ __forceinline__ int v_chunk(int row, int chunk) { return CH >= 8 ? chunk ^ (row & 6) : chunk ^ ((row >> 1) & 3); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Barriers of two of the CTA's warps: one waits, the other one only reports.
+enum { kGiven1 = 1, kGiven2, kGiven3, kTaken2, kTaken3 };
+__device__ __forceinline__ void barrier_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+
+// A place in the sequence of units: unit kb of the nb units of segment (b, hw), whose sequence has n keys.
+struct Cursor {
+    int b, hw, kb, nb, n, left;    // left: units of the CTA from here on
+    __device__ __forceinline__ void enter(const CachedAttnParams& p, int sequence) {
+        b = sequence;
+        nb = units_of(p, b, &n);
+    }
+    // To the start of the next segment, if the CTA has units there.
+    __device__ __forceinline__ void next(const CachedAttnParams& p, int W) {
+        kb = 0;
+        if (++hw == W) {
+            hw = 0;
+            if (left > 0) enter(p, b + 1);
+        }
+    }
+};
 
 template <typename T, bool QUANT, int D, int NT>
-__global__ void __launch_bounds__(128) cached_attention_kernel(const CachedAttnParams p) {
+__global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attention_kernel(const CachedAttnParams p) {
     using M = typename std::conditional<QUANT, fp16, T>::type;    // operand type of the products
-    constexpr int ROW = D * (QUANT ? 1 : 2);                      // bytes of a cache row
-    constexpr int KC = ROW / 64;                                  // 16-byte chunks of a key row per lane
+    using R = Ring<QUANT, D, NT>;
+    constexpr int ROW = R::kRow;
+    constexpr int CH = ROW / 16;                                  // 16-byte chunks of a row
+    constexpr int KC = ROW / 64;                                  // chunks of a key row per lane
     constexpr int VW = ROW / 32;                                  // 4-byte words of a value row per lane
     constexpr int KS = D / 16;                                    // contraction steps of S^T = tiles of 16 columns of O
     constexpr int NQ = 8 * NT;
-    __shared__ float sh_o[4][NQ][D + 4];
-    __shared__ float sh_m[4][NQ], sh_l[4][NQ], sh_ref[4];
-    __shared__ int64_t sh_sum[4], sh_pos[2];
+    constexpr int ES = QUANT ? 1 : 2;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int sh_sum[4], sh_pos[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     grid_launch_dependents();
     grid_dependency_wait();
 
     // ---- this CTA's range of units ----
-    const int64_t W = static_cast<int64_t>(p.Hkv) * p.tiles;
-    const int64_t per = (p.B + 127) / 128;
-    const int64_t b_lo = min(static_cast<int64_t>(p.B), threadIdx.x * per), b_hi = min(static_cast<int64_t>(p.B), b_lo + per);
-    int64_t mine = 0, n = 0;
-    for (int64_t i = b_lo; i < b_hi; ++i) mine += units_of(p, i, &n);
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-    }
-    if (lane == 31) sh_sum[warp] = incl;
-    __syncthreads();
-    int64_t excl = incl - mine, all = 0;
-    for (int w = 0; w < 4; ++w) {
-        if (w < warp) excl += sh_sum[w];
-        all += sh_sum[w];
-    }
-    if (blockIdx.x == 0 && p.before != nullptr) {
-        int64_t x = excl;
-        for (int64_t i = b_lo; i < b_hi; ++i) {
-            p.before[i] = x;
-            x += units_of(p, i, &n);
-        }
-        if (threadIdx.x == 0) p.before[p.B] = all;
-    }
-    const int64_t total = all * W;
-    const int64_t ctas = ctas_of(p, total);
-    if (blockIdx.x >= ctas) return;
-    int64_t u = total * blockIdx.x / ctas;
-    const int64_t u_end = total * (blockIdx.x + 1) / ctas;
-    if (u >= u_end) return;
-    if (u >= excl * W && u < (excl + mine) * W) {
-        int64_t x = excl;
-        for (int64_t i = b_lo; i < b_hi; ++i) {
-            const int64_t nb = units_of(p, i, &n);
-            if (u < (x + nb) * W) {
-                sh_pos[0] = i;
-                sh_pos[1] = x;
-                break;
-            }
-            x += nb;
-        }
-    }
-    __syncthreads();
-    int64_t b = sh_pos[0];
-    int64_t nb = units_of(p, b, &n);
-    int64_t hw, kb;
+    const int W = p.Hkv * p.tiles;
+    Cursor at;
     {
-        const int64_t r = u - sh_pos[1] * W;
-        hw = r / nb;
-        kb = r - hw * nb;
-    }
-    if (p.whole && kb != 0) {   // whole segments: those that start in the range
-        u += nb - kb;
-        kb = 0;
-        ++hw;
+        const int per = (p.B + 127) / 128;
+        const int b_lo = min(p.B, static_cast<int>(threadIdx.x) * per), b_hi = min(p.B, b_lo + per);
+        int mine = 0, n = 0;
+        for (int i = b_lo; i < b_hi; ++i) mine += kStart + units_of(p, i, &n);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        if (lane == 31) sh_sum[warp] = incl;
+        __syncthreads();
+        int excl = incl - mine, all = 0;
+        for (int w = 0; w < 4; ++w) {
+            if (w < warp) excl += sh_sum[w];
+            all += sh_sum[w];
+        }
+        if (blockIdx.x == 0 && p.before != nullptr) {
+            int x = excl;
+            for (int i = b_lo; i < b_hi; ++i) {
+                p.before[i] = x;
+                x += kStart + units_of(p, i, &n);
+            }
+            if (threadIdx.x == 0) p.before[p.B] = all;
+        }
+        const int total = all * W, ctas = ctas_of(p, total);
+        if (blockIdx.x >= ctas) return;
+        const int x0 = place_of(total, blockIdx.x, ctas), x1 = place_of(total, blockIdx.x + 1, ctas);
+        // the sequences that hold x0 and x1 (x1 = total: behind the last one)
+        if (threadIdx.x == 0) {
+            sh_pos[2] = p.B;
+            sh_pos[3] = all;
+        }
+        __syncthreads();
+        const int lo = excl * W, hi = (excl + mine) * W;
+        if ((x0 >= lo && x0 < hi) || (x1 >= lo && x1 < hi)) {
+            int x = excl;
+            for (int i = b_lo; i < b_hi; ++i) {
+                const int w = kStart + units_of(p, i, &n);
+                if (x0 >= x * W && x0 < (x + w) * W) {
+                    sh_pos[0] = i;
+                    sh_pos[1] = x;
+                }
+                if (x1 >= x * W && x1 < (x + w) * W) {
+                    sh_pos[2] = i;
+                    sh_pos[3] = x;
+                }
+                x += w;
+            }
+        }
+        __syncthreads();
+        // units in front of a place: the places in front of its segment without the segments' own, and what the segment adds
+        at.enter(p, sh_pos[0]);
+        const int r0 = x0 - sh_pos[1] * W;
+        at.hw = r0 / (kStart + at.nb);
+        at.kb = max(0, r0 - at.hw * (kStart + at.nb) - kStart);
+        const int front0 = (sh_pos[1] - kStart * at.b) * W + at.hw * at.nb + at.kb;
+        int front1 = (all - kStart * p.B) * W, over = 0, nb1 = 0;
+        if (sh_pos[2] < p.B) {
+            nb1 = units_of(p, sh_pos[2], &n);
+            const int r1 = x1 - sh_pos[3] * W, hw1 = r1 / (kStart + nb1);
+            over = max(0, r1 - hw1 * (kStart + nb1) - kStart);
+            front1 = (sh_pos[3] - kStart * sh_pos[2]) * W + hw1 * nb1 + over;
+        }
+        at.left = front1 - front0;
+        if (p.whole) {   // whole segments, those whose first unit is in the range
+            const int skip = at.kb == 0 ? 0 : at.nb - at.kb;
+            at.left += (over == 0 ? 0 : nb1 - over) - skip;
+            if (skip != 0) at.next(p, W);
+        }
+        if (at.left <= 0) return;
     }
 
-    while (u < u_end) {
-        if (hw == W) {
-            hw = 0;
-            ++b;
-            nb = units_of(p, b, &n);
+    // ---- the copies, up to `kStages` tiles ahead of the products, across the ends of segments ----
+    // Keys and values go in copy groups of their own, so that a tile's key rows are replaced as soon as its scores are there.
+    uint8_t* ring = smem + warp * R::kWarp;
+    constexpr int RPC = 512 / ROW, NC = 16 / RPC;     // rows a copy instruction of the warp covers; copies of a tile
+    const int my_row = lane / CH, my_chunk = lane % CH;
+    const uint32_t k_dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + my_row * ROW + k_chunk<CH>(my_row, my_chunk) * 16;
+    const uint32_t v_dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + R::kKeys + my_row * ROW;
+    const int64_t k_pitch = p.k_sl * ES, v_pitch = p.v_sl * ES;
+    Cursor ahead = at;
+    int ahead_run = 0;                                // units of the current segment still to be copied
+    int ahead_k0 = 0;                                 // first key of the warp's next tile
+    const uint8_t *k_src = nullptr, *v_src = nullptr; // that key's row, this lane's part of it
+    const float* s_src = nullptr;
+    uint32_t put = 0;                                 // byte offset of the stage to fill
+    auto copy_keys = [&]() {
+        if (ahead_run == 0 && ahead.left > 0) {       // the next segment
+            ahead_run = min(ahead.nb - ahead.kb, ahead.left);
+            ahead_k0 = ahead.kb * kUnit + warp * 16;
+            const int hk = ahead.hw / p.tiles;
+            k_src = static_cast<const uint8_t*>(p.k) + (ahead.b * p.k_sb + hk * p.k_sh) * ES + (ahead_k0 + my_row) * k_pitch + my_chunk * 16;
+            v_src = static_cast<const uint8_t*>(p.v) + (ahead.b * p.v_sb + hk * p.v_sh) * ES + (ahead_k0 + my_row) * v_pitch + my_chunk * 16;
+            if (QUANT) s_src = (lane < 16 ? p.ks + ahead.b * p.ks_sb + hk * p.ks_sh : p.vs + ahead.b * p.vs_sb + hk * p.vs_sh) + ahead_k0;
         }
-        const int hk = static_cast<int>(hw / p.tiles), tile = static_cast<int>(hw - static_cast<int64_t>(hk) * p.tiles);
+        if (ahead_run > 0 && ahead_k0 < ahead.n) {
+            const int last = ahead.n - 1 - ahead_k0;  // rows behind the sequence are replaced by its last one (their scores become -inf)
+            if (last >= 15) {
+                const uint8_t* src = k_src;
+#pragma unroll
+                for (int i = 0; i < NC; ++i, src += RPC * k_pitch) copy16(k_dst + put + i * 512, src);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NC; ++i) copy16(k_dst + put + i * 512, k_src + (min(my_row + i * RPC, last) - my_row) * k_pitch);
+            }
+            if (QUANT) copy4(k_dst + put - my_row * ROW - k_chunk<CH>(my_row, my_chunk) * 16 + 16 * ROW + lane * 4, s_src + min(lane & 15, last));
+        }
+        copies_commit();
+    };
+    auto copy_values = [&]() {
+        if (ahead_run > 0) {
+            if (ahead_k0 < ahead.n) {
+                const int last = ahead.n - 1 - ahead_k0;
+                if (last >= 15) {
+                    const uint8_t* src = v_src;
+#pragma unroll
+                    for (int i = 0; i < NC; ++i, src += RPC * v_pitch) copy16(v_dst + put + i * 512 + v_chunk<CH>(my_row + i * RPC, my_chunk) * 16, src);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NC; ++i)
+                        copy16(v_dst + put + i * 512 + v_chunk<CH>(my_row + i * RPC, my_chunk) * 16, v_src + (min(my_row + i * RPC, last) - my_row) * v_pitch);
+                }
+            }
+            ahead_k0 += kUnit;
+            k_src += kUnit * k_pitch;
+            v_src += kUnit * v_pitch;
+            if (QUANT) s_src += kUnit;
+            --ahead.left;
+            if (--ahead_run == 0) ahead.next(p, W);
+        }
+        copies_commit();
+        put += R::kStage;
+        if (put == R::kWarp) put = 0;
+    };
+#pragma unroll
+    for (int i = 0; i < R::kStages; ++i) {
+        copy_keys();
+        copy_values();
+    }
+
+    float* join = reinterpret_cast<float*>(smem + 4 * R::kWarp);
+    // A segment's query rows, as they come: this lane's 16-byte chunks of row g (of each group of eight). Loaded before the previous
+    // segment is finished.
+    constexpr int QW = D / 32;
+    uint4 qw[NT][QW];
+    auto load_queries = [&]() {
+        const int hk = at.hw / p.tiles, tile = at.hw - hk * p.tiles;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int q = tile * NQ + nt * 8 + g;
+            const T* src = static_cast<const T*>(p.q) + at.b * p.q_sb + static_cast<int64_t>(hk * p.group + q) * p.q_sh;
+#pragma unroll
+            for (int i = 0; i < QW; ++i) {
+                const int e = QUANT ? (i >> 1) * 64 + t * 16 + (i & 1) * 8 : i * 32 + t * 8;
+                qw[nt][i] = q < p.group ? *reinterpret_cast<const uint4*>(src + e) : make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
+    load_queries();
+    uint32_t get = 0;
+    bool first = true;
+    while (at.left > 0) {
+        const int b = at.b, hw = at.hw, n = at.n;
+        const int hk = hw / p.tiles, tile = hw - hk * p.tiles;
         const int row0 = hk * p.group + tile * NQ;             // first query head of the segment
         const int rows = min(NQ, p.group - tile * NQ);
-        const int64_t kb_first = kb;
-        const int64_t kb_end = p.whole ? nb : min(nb, kb + (u_end - u));
-        u += p.whole ? nb : kb_end - kb;
+        const int run = min(at.nb - at.kb, at.left);
+        const bool complete = at.kb == 0 && run == at.nb, from_start = at.kb == 0;
+        int k0 = at.kb * kUnit + warp * 16;
+        at.left -= run;
+        at.next(p, W);
 
         // ---- queries as the second operand of S^T: column g, the contracted index in the order of the key rows ----
         uint32_t qf[NT][KS][2];
         float sl[NT][2];                                       // softmax scale of columns 2t and 2t + 1, in log2
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const bool have = nt * 8 + g < rows;
-            const T* src = static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(row0 + nt * 8 + g) * p.q_sh;
             float back = 1.f;
             if constexpr (QUANT) {
-                uint4 w[KC][2];
-#pragma unroll
-                for (int c = 0; c < KC; ++c) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) w[c][i] = have ? *reinterpret_cast<const uint4*>(src + c * 64 + t * 16 + i * 8) : make_uint4(0, 0, 0, 0);
-                }
                 float up = 1.f;
                 if constexpr (std::is_same<T, bf16>::value) {
                     // bf16 reaches beyond fp16: the row is multiplied by the power of two that takes its largest value to
                     // [2^14, 2^15). Exact, except for values below 2^-28 of that largest one.
                     float top = 0.f;
 #pragma unroll
-                    for (int c = 0; c < KC; ++c) {
+                    for (int i = 0; i < QW; ++i) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float2 x = Pair<T>::widen(word(w[c][i], j));
-                                top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 x = Pair<T>::widen(word(qw[nt][i], j));
+                            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
                         }
                     }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -239,23 +391,18 @@ __global__ void __launch_bounds__(128) cached_attention_kernel(const CachedAttnP
                     back = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
                 }
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
+                for (int j = 0; j < KS; ++j) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint4 ww = w[c][j >> 1];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t x = word(ww, (j & 1) * 2 + i);
-                            qf[nt][c * 4 + j][i] = std::is_same<T, bf16>::value ? Pair<fp16>::narrow(mul2(Pair<T>::widen(x), make_float2(up, up))) : x;
-                        }
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t x = word(qw[nt][j >> 1], (j & 1) * 2 + i);
+                        qf[nt][j][i] = std::is_same<T, bf16>::value ? Pair<fp16>::narrow(mul2(Pair<T>::widen(x), make_float2(up, up))) : x;
                     }
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const uint4 w = have ? *reinterpret_cast<const uint4*>(src + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
-                    qf[nt][c * 2][0] = w.x; qf[nt][c * 2][1] = w.y;
-                    qf[nt][c * 2 + 1][0] = w.z; qf[nt][c * 2 + 1][1] = w.w;
+                for (int j = 0; j < KS; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) qf[nt][j][i] = word(qw[nt][j >> 1], (j & 1) * 2 + i);
                 }
             }
             sl[nt][0] = p.scale_log2 * __shfl_sync(0xffffffffu, back, t * 8);
@@ -266,341 +413,374 @@ __global__ void __launch_bounds__(128) cached_attention_kernel(const CachedAttnP
         float vref = 0.f, ivref = 0.f;   // QUANT: P is held relative to the largest value scale so far (rounded up to a power of two)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = -INFINITY;
+            m[nt][0] = m[nt][1] = kLowest;
             l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
         }
 
-        const char* kbase = static_cast<const char*>(p.k) + (b * p.k_sb + hk * p.k_sh) * (QUANT ? 1 : 2) + t * 16;
-        const char* vbase = static_cast<const char*>(p.v) + (b * p.v_sb + hk * p.v_sh) * (QUANT ? 1 : 2) + g * (VW * 4 > 16 ? 16 : VW * 4);
-        const float* ksb = QUANT ? p.ks + b * p.ks_sb + hk * p.ks_sh : nullptr;
-        const float* vsb = QUANT ? p.vs + b * p.vs_sb + hk * p.vs_sh : nullptr;
-        const int64_t k_row = p.k_sl * (QUANT ? 1 : 2), v_row = p.v_sl * (QUANT ? 1 : 2);
-        // The last row a lane may read: rows behind the sequence are replaced by its last one and their scores by -inf
-        const int64_t last = n - 1;
-        uint4 kw[2][KC];
-        uint32_t vw[4][VW];
-        float ksc[2], vsc[2];
-        auto load_k = [&](int64_t k0) {
+#pragma unroll 1
+        for (int u = 0; u < run; ++u, k0 += kUnit) {
+            copies_wait<2 * R::kStages - 1>();
+            __syncwarp();
+            uint32_t pb[NT][2];
+            const uint8_t* stage = ring + get;
+            if (k0 < n) {
+                float s[NT][4], s2[NT][4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t row = min(k0 + g + 8 * r, last);
+                for (int c = 0; c < KC; ++c) {
+                    const uint4 kw0 = *reinterpret_cast<const uint4*>(stage + g * ROW + k_chunk<CH>(g, t + 4 * c) * 16);
+                    const uint4 kw1 = *reinterpret_cast<const uint4*>(stage + (g + 8) * ROW + k_chunk<CH>(g + 8, t + 4 * c) * 16);
+                    constexpr int PER = QUANT ? 4 : 2;
 #pragma unroll
-                for (int c = 0; c < KC; ++c) kw[r][c] = ldg16_once(kbase + row * k_row + c * 64);
-                if (QUANT) {
-                    ksc[r] = ksb[row];
-                    vsc[r] = vsb[row];
-                }
-            }
-        };
-        auto load_v = [&](int64_t k0) {
+                    for (int j = 0; j < PER; ++j) {
+                        const int i = c * PER + j;
+                        uint32_t a[4];
+                        if constexpr (QUANT) {
+                            const uint32_t w0 = word(kw0, j) ^ 0x80808080u, w1 = word(kw1, j) ^ 0x80808080u;
+                            a[0] = codes_to_half2<0x4140>(w0); a[1] = codes_to_half2<0x4140>(w1);
+                            a[2] = codes_to_half2<0x4342>(w0); a[3] = codes_to_half2<0x4342>(w1);
+                        } else {
+                            a[0] = word(kw0, 2 * j); a[1] = word(kw1, 2 * j);
+                            a[2] = word(kw0, 2 * j + 1); a[3] = word(kw1, 2 * j + 1);
+                        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = min(k0 + 2 * t + (r & 1) + 8 * (r >> 1), last);
-                const char* src = vbase + row * v_row;
-                if constexpr (VW == 2) {
-                    const uint2 x = ldg8_once(src);
-                    vw[r][0] = x.x; vw[r][1] = x.y;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < VW / 4; ++c) {
-                        const uint4 x = ldg16_once(src + c * 128);
-                        vw[r][4 * c] = x.x; vw[r][4 * c + 1] = x.y; vw[r][4 * c + 2] = x.z; vw[r][4 * c + 3] = x.w;
-                    }
-                }
-            }
-        };
-        int64_t k0 = kb * kUnit + warp * 16;
-        const int64_t k_stop = min(kb_end * kUnit, n);
-        if (k0 < k_stop) {
-            load_k(k0);
-            load_v(k0);
-        }
-        for (; k0 < k_stop; k0 += kUnit) {
-            const bool more = k0 + kUnit < k_stop;
-            float s[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                uint32_t a[4];
-                if constexpr (QUANT) {
-                    const uint32_t w0 = word(kw[0][i >> 2], i & 3) ^ 0x80808080u, w1 = word(kw[1][i >> 2], i & 3) ^ 0x80808080u;
-                    a[0] = codes_to_half2<0x4140>(w0); a[1] = codes_to_half2<0x4140>(w1);
-                    a[2] = codes_to_half2<0x4342>(w0); a[3] = codes_to_half2<0x4342>(w1);
-                } else {
-                    a[0] = word(kw[0][i >> 1], (i & 1) * 2); a[1] = word(kw[1][i >> 1], (i & 1) * 2);
-                    a[2] = word(kw[0][i >> 1], (i & 1) * 2 + 1); a[3] = word(kw[1][i >> 1], (i & 1) * 2 + 1);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816<M>(s[nt], a, qf[nt][i][0], qf[nt][i][1]);
-            }
-            const float ks0 = QUANT ? ksc[0] : 1.f, ks1 = QUANT ? ksc[1] : 1.f;
-            float vs0 = 1.f, vs1 = 1.f;
-            if (QUANT) {
-                vs0 = vsc[0];
-                vs1 = vsc[1];
-            }
-            if (more) load_k(k0 + kUnit);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                s[nt][0] *= ks0 * sl[nt][0]; s[nt][1] *= ks0 * sl[nt][1];
-                s[nt][2] *= ks1 * sl[nt][0]; s[nt][3] *= ks1 * sl[nt][1];
-            }
-            if (k0 + 16 > n) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (k0 + g >= n) s[nt][0] = s[nt][1] = -INFINITY;
-                    if (k0 + g + 8 >= n) s[nt][2] = s[nt][3] = -INFINITY;
-                }
-            }
-            bool grow = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) grow |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + kGrow || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + kGrow;
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float x = fmaxf(s[nt][c], s[nt][2 + c]);
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        x = fmaxf(x, m[nt][c]);
-                        const float f = m[nt][c] == -INFINITY ? 0.f : exp2_approx(m[nt][c] - x);
-                        m[nt][c] = x;
-                        l[nt][c] *= f;
-#pragma unroll
-                        for (int i = 0; i < KS; ++i) {
-                            acc[nt][i][c] *= f;
-                            acc[nt][i][2 + c] *= f;
+                        for (int nt = 0; nt < NT; ++nt) {   // two chains: half the latency
+                            if (i < 2) mma16816_first<M>(i == 0 ? s[nt] : s2[nt], a, qf[nt][i][0], qf[nt][i][1]);
+                            else mma16816<M>((i & 1) ? s2[nt] : s[nt], a, qf[nt][i][0], qf[nt][i][1]);
                         }
                     }
                 }
-            }
-            if (QUANT) {
-                const uint32_t vm = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(vs0), fabsf(vs1))));
-                if (vm > __float_as_uint(vref) && vm < 0x7f000000u) {
-                    const float up = __uint_as_float((vm & 0x7f800000u) + 0x00800000u);
-                    ivref = 1.f / up;
-                    const float f = vref * ivref;
-                    vref = up;
+                float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f;
+                if (QUANT) {
+                    const float* sc = reinterpret_cast<const float*>(stage + 16 * ROW);
+                    ks0 = sc[g]; ks1 = sc[g + 8];
+                    vs0 = sc[16 + g]; vs1 = sc[24 + g];
+                }
+                __syncwarp();       // every lane has read the key rows: the next ones go there
+                copy_keys();
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[nt][0] = (s[nt][0] + s2[nt][0]) * (ks0 * sl[nt][0]); s[nt][1] = (s[nt][1] + s2[nt][1]) * (ks0 * sl[nt][1]);
+                    s[nt][2] = (s[nt][2] + s2[nt][2]) * (ks1 * sl[nt][0]); s[nt][3] = (s[nt][3] + s2[nt][3]) * (ks1 * sl[nt][1]);
+                }
+                if (k0 + 16 > n) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (k0 + g >= n) s[nt][0] = s[nt][1] = -INFINITY;
+                        if (k0 + g + 8 >= n) s[nt][2] = s[nt][3] = -INFINITY;
+                    }
+                }
+                bool grow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) grow |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + kGrow || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + kGrow;
+                if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int i = 0; i < KS; ++i) {
-                            acc[nt][i][0] *= f; acc[nt][i][1] *= f;
-                            acc[nt][i][2] *= f; acc[nt][i][3] *= f;
+                        for (int c = 0; c < 2; ++c) {
+                            float x = fmaxf(s[nt][c], s[nt][2 + c]);
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            x = fmaxf(x, m[nt][c]);
+                            const float f = exp2_approx(m[nt][c] - x);
+                            m[nt][c] = x;
+                            l[nt][c] *= f;
+#pragma unroll
+                            for (int i = 0; i < KS; ++i) {
+                                acc[nt][i][c] *= f;
+                                acc[nt][i][2 + c] *= f;
+                            }
                         }
                     }
                 }
-                vs0 *= ivref;
-                vs1 *= ivref;
-            }
-            uint32_t pb[NT][2];
+                if (QUANT) {
+                    const uint32_t vm = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(vs0), fabsf(vs1))));
+                    if (vm > __float_as_uint(vref) && vm < 0x7f000000u) {
+                        const float up = __uint_as_float((vm & 0x7f800000u) + 0x00800000u);
+                        ivref = 1.f / up;
+                        const float f = vref * ivref;
+                        vref = up;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-                const float e0 = exp2_approx(s[nt][0] - m0), e1 = exp2_approx(s[nt][1] - m1);
-                const float e2 = exp2_approx(s[nt][2] - m0), e3 = exp2_approx(s[nt][3] - m1);
-                l[nt][0] += e0 + e2;
-                l[nt][1] += e1 + e3;
-                pb[nt][0] = transpose8x8(Pair<M>::narrow(make_float2(e0 * vs0, e1 * vs0)));
-                pb[nt][1] = transpose8x8(Pair<M>::narrow(make_float2(e2 * vs1, e3 * vs1)));
-            }
+                        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                uint32_t a[4];
-                if constexpr (QUANT) {
-                    constexpr int kLo = 0x5140, kHi = 0x7362;
-                    const uint32_t w0 = __byte_perm(vw[0][i >> 1] ^ 0x80808080u, vw[1][i >> 1] ^ 0x80808080u, (i & 1) ? kHi : kLo);
-                    const uint32_t w1 = __byte_perm(vw[2][i >> 1] ^ 0x80808080u, vw[3][i >> 1] ^ 0x80808080u, (i & 1) ? kHi : kLo);
-                    a[0] = codes_to_half2<0x4140>(w0); a[1] = codes_to_half2<0x4342>(w0);
-                    a[2] = codes_to_half2<0x4140>(w1); a[3] = codes_to_half2<0x4342>(w1);
-                } else {
-                    a[0] = __byte_perm(vw[0][i], vw[1][i], 0x5410); a[1] = __byte_perm(vw[0][i], vw[1][i], 0x7632);
-                    a[2] = __byte_perm(vw[2][i], vw[3][i], 0x5410); a[3] = __byte_perm(vw[2][i], vw[3][i], 0x7632);
+                            for (int i = 0; i < KS; ++i) {
+                                acc[nt][i][0] *= f; acc[nt][i][1] *= f;
+                                acc[nt][i][2] *= f; acc[nt][i][3] *= f;
+                            }
+                        }
+                    }
+                    vs0 *= ivref;
+                    vs1 *= ivref;
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816<M>(acc[nt][i], a, pb[nt][0], pb[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float e0 = exp2_approx(s[nt][0] - m[nt][0]), e1 = exp2_approx(s[nt][1] - m[nt][1]);
+                    const float e2 = exp2_approx(s[nt][2] - m[nt][0]), e3 = exp2_approx(s[nt][3] - m[nt][1]);
+                    l[nt][0] += e0 + e2;
+                    l[nt][1] += e1 + e3;
+                    pb[nt][0] = transpose8x8(Pair<M>::narrow(make_float2(e0 * vs0, e1 * vs0)));
+                    pb[nt][1] = transpose8x8(Pair<M>::narrow(make_float2(e2 * vs1, e3 * vs1)));
+                }
+            } else {
+                copy_keys();
             }
-            if (more) load_v(k0 + kUnit);
-        }
-
-        // ---- join the four warps ----
+            copies_wait<2 * R::kStages - 1>();
+            __syncwarp();
+            if (k0 < n) {
+                const uint8_t* vt = stage + R::kKeys;
+                uint32_t vw[4][VW];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 2 * t + (r & 1) + 8 * (r >> 1);
+                    if constexpr (VW == 2) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(vt + row * ROW + v_chunk<CH>(row, g >> 1) * 16 + (g & 1) * 8);
+                        vw[r][0] = x.x; vw[r][1] = x.y;
+                    } else {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x = l[nt][c];
-                x += __shfl_xor_sync(0xffffffffu, x, 4);
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                const int q = nt * 8 + 2 * t + c;
-                if (g == 0) {
-                    sh_m[warp][q] = m[nt][c];
-                    sh_l[warp][q] = x;
+                        for (int c = 0; c < VW / 4; ++c) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(vt + row * ROW + v_chunk<CH>(row, g + 8 * c) * 16);
+                            vw[r][4 * c] = x.x; vw[r][4 * c + 1] = x.y; vw[r][4 * c + 2] = x.z; vw[r][4 * c + 3] = x.w;
+                        }
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
-                    // columns 2i and 2i + 1 of the lane's value chunk(s)
-                    const int e = VW > 4 ? ((2 * i) >> 3) * 64 + g * 8 + ((2 * i) & 7) : g * KS * 2 + 2 * i;
-                    *reinterpret_cast<float2*>(&sh_o[warp][q][e]) = make_float2(acc[nt][i][c], acc[nt][i][2 + c]);
+                    uint32_t a[4];
+                    if constexpr (QUANT) {
+                        const uint32_t w0 = __byte_perm(vw[0][i >> 1], vw[1][i >> 1], (i & 1) ? 0x7362 : 0x5140) ^ 0x80808080u;
+                        const uint32_t w1 = __byte_perm(vw[2][i >> 1], vw[3][i >> 1], (i & 1) ? 0x7362 : 0x5140) ^ 0x80808080u;
+                        a[0] = codes_to_half2<0x4140>(w0); a[1] = codes_to_half2<0x4342>(w0);
+                        a[2] = codes_to_half2<0x4140>(w1); a[3] = codes_to_half2<0x4342>(w1);
+                    } else {
+                        a[0] = __byte_perm(vw[0][i], vw[1][i], 0x5410); a[1] = __byte_perm(vw[0][i], vw[1][i], 0x7632);
+                        a[2] = __byte_perm(vw[2][i], vw[3][i], 0x5410); a[3] = __byte_perm(vw[2][i], vw[3][i], 0x7632);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816<M>(acc[nt][i], a, pb[nt][0], pb[nt][1]);
+                }
+            }
+            get += R::kStage;
+            if (get == R::kWarp) get = 0;
+            __syncwarp();           // and the value rows
+            copy_values();
+        }
+
+        if (at.left > 0) load_queries();
+        // ---- join the four warps: 2 and 3 into 0 and 1, then 1 into 0. A lane's values meet the same lane's ----
+        if (!QUANT) vref = 1.f;
+        auto put_slot = [&](float* slot) {
+            float4* d = reinterpret_cast<float4*>(slot) + lane;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) d[(nt * (KS + 1) + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
+                d[(nt * (KS + 1) + KS) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
+            }
+            d[NT * (KS + 1) * 32] = make_float4(vref, 0.f, 0.f, 0.f);
+        };
+        auto add_slot = [&](const float* slot) {
+            const float4* d = reinterpret_cast<const float4*>(slot) + lane;
+            const float ref = d[NT * (KS + 1) * 32].x, top = fmaxf(vref, ref);
+            const float ra = top > 0.f ? vref / top : 0.f, rb = top > 0.f ? ref / top : 0.f;
+            vref = top;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float4 x = d[(nt * (KS + 1) + KS) * 32];
+                const float m0 = fmaxf(m[nt][0], x.x), m1 = fmaxf(m[nt][1], x.y);
+                const float fa0 = exp2_approx(m[nt][0] - m0), fa1 = exp2_approx(m[nt][1] - m1), fb0 = exp2_approx(x.x - m0), fb1 = exp2_approx(x.y - m1);
+                l[nt][0] = l[nt][0] * fa0 + x.z * fb0;
+                l[nt][1] = l[nt][1] * fa1 + x.w * fb1;
+                m[nt][0] = m0;
+                m[nt][1] = m1;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const float4 o = d[(nt * (KS + 1) + i) * 32];
+                    acc[nt][i][0] = acc[nt][i][0] * (fa0 * ra) + o.x * (fb0 * rb);
+                    acc[nt][i][1] = acc[nt][i][1] * (fa1 * ra) + o.y * (fb1 * rb);
+                    acc[nt][i][2] = acc[nt][i][2] * (fa0 * ra) + o.z * (fb0 * rb);
+                    acc[nt][i][3] = acc[nt][i][3] * (fa1 * ra) + o.w * (fb1 * rb);
+                }
+            }
+        };
+        // Pairwise barriers: who only gives goes on to the next segment. kTaken: warp 0 has read what warp 2 (3) gave the last time.
+        float* const slot0 = join;
+        float* const slot1 = join + R::kJoinFloats * 32;
+        if (warp >= 2) {
+            if (!first) barrier_sync(warp == 2 ? kTaken2 : kTaken3);
+            put_slot(warp == 2 ? slot0 : slot1);
+            barrier_arrive(warp == 2 ? kGiven2 : kGiven3);
+        } else if (warp == 1) {
+            barrier_sync(kGiven3);
+            add_slot(slot1);
+            __syncwarp();
+            put_slot(slot1);
+            barrier_arrive(kGiven1);
+        } else {
+            barrier_sync(kGiven2);
+            add_slot(slot0);
+            if (at.left > 0) barrier_arrive(kTaken2);
+            barrier_sync(kGiven1);
+            add_slot(slot1);
+            if (at.left > 0) barrier_arrive(kTaken3);
+            const bool last_word = complete && p.prefix.splits == 0;
+            const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + static_cast<int64_t>(b) * W + hw : 2 * static_cast<int64_t>(blockIdx.x) + (from_start ? 1 : 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float ll = l[nt][c];
+                    ll += __shfl_xor_sync(0xffffffffu, ll, 4);
+                    ll += __shfl_xor_sync(0xffffffffu, ll, 8);
+                    ll += __shfl_xor_sync(0xffffffffu, ll, 16);
+                    const int q = nt * 8 + 2 * t + c;
+                    if (q >= rows) continue;
+                    // a lane holds runs of 8 (int8 rows of 128: 16) neighbouring columns
+                    if (last_word) {
+                        const float f = ll == 0.f ? 0.f : vref / ll;
+                        T* dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(row0 + q) * p.o_sh;
+#pragma unroll
+                        for (int i = 0; i < KS; i += 4) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) w[j] = Pair<T>::narrow(make_float2(acc[nt][i + j][c] * f, acc[nt][i + j][2 + c] * f));
+                            *reinterpret_cast<uint4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 : g * KS * 2 + 2 * i)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        if (g == 0 && p.lse != nullptr)
+                            p.lse[b * p.lse_sb + static_cast<int64_t>(row0 + q) * p.lse_sh] = ll == 0.f ? -INFINITY : (m[nt][c] + log2f(ll)) * 0.6931471805599453f;
+                    } else {
+                        float* dst = p.part_o + (slot * NQ + q) * D;
+#pragma unroll
+                        for (int i = 0; i < KS; i += 2) {
+                            *reinterpret_cast<float4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 + (2 * i & 7) : g * KS * 2 + 2 * i)) =
+                                make_float4(acc[nt][i][c] * vref, acc[nt][i][2 + c] * vref, acc[nt][i + 1][c] * vref, acc[nt][i + 1][2 + c] * vref);
+                        }
+                        if (g == 0) p.part_ml[slot * NQ + q] = make_float2(m[nt][c], ll);
+                    }
                 }
             }
         }
-        if (lane == 0) sh_ref[warp] = QUANT ? vref : 1.f;
-        __syncthreads();
-        const bool complete = p.whole || (kb_first == 0 && kb_end == nb);
-        for (int item = threadIdx.x; item < rows * (D / 4); item += 128) {
-            const int q = item / (D / 4), c = (item - q * (D / 4)) * 4;
-            float mm = fmaxf(fmaxf(sh_m[0][q], sh_m[1][q]), fmaxf(sh_m[2][q], sh_m[3][q]));
-            const float base = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = exp2_approx(sh_m[w][q] - base), fo = f * sh_ref[w];
-                ll += sh_l[w][q] * f;
-                const float4 x = *reinterpret_cast<const float4*>(&sh_o[w][q][c]);
-                o.x += x.x * fo; o.y += x.y * fo; o.z += x.z * fo; o.w += x.w * fo;
-            }
-            if (complete && p.prefix.splits == 0) {
-                const float inv = ll == 0.f ? 0.f : 1.f / ll;
-                T* dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(row0 + q) * p.o_sh + c;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(Pair<T>::narrow(make_float2(o.x * inv, o.y * inv)), Pair<T>::narrow(make_float2(o.z * inv, o.w * inv)));
-                if (c == 0 && p.lse != nullptr)
-                    p.lse[b * p.lse_sb + static_cast<int64_t>(row0 + q) * p.lse_sh] = ll == 0.f ? -INFINITY : (base + log2f(ll)) * 0.6931471805599453f;
-            } else {
-                const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + b * W + hw : 2 * static_cast<int64_t>(blockIdx.x) + (kb_first == 0 ? 1 : 0);
-                *reinterpret_cast<float4*>(p.part_o + (slot * NQ + q) * D + c) = o;
-                if (c == 0) p.part_ml[slot * NQ + q] = make_float2(mm, ll);
-            }
-        }
-        __syncthreads();
-        kb = kb_end;
-        if (kb == nb) {
-            kb = 0;
-            ++hw;
-        }
+        first = false;
     }
+    copies_wait<0>();
 }
 
-// Joins the pieces of one (sequence, query head): those of the prefix, if there is one, and those of the own keys.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) cached_attention_join_kernel(const CachedAttnParams p, int nq) {
-    __shared__ float red[4];
-    __shared__ float sh_l[4];
-    __shared__ float sh_o[4][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t b = blockIdx.x / p.Hq;
-    const int h = static_cast<int>(blockIdx.x - b * p.Hq), hk = h / p.group, in_group = h - hk * p.group;
-    const int tile = in_group / nq, q = in_group - tile * nq;
-    const int64_t W = static_cast<int64_t>(p.Hkv) * p.tiles, hw = static_cast<int64_t>(hk) * p.tiles + tile;
+// Joins the pieces of one (sequence, query head): those of the prefix, if there is one, and those of the own keys. WARPS warps take a
+// row: a CTA's sixteen where rows are few and have many pieces, one where rows are many. A warp keeps a running maximum over its
+// pieces, so that maxima and outputs are fetched together.
+template <typename T, int D, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attention_join_kernel(const CachedAttnParams p, int nq) {
+    constexpr int N = D / 32;
+    __shared__ float sh_m[WARPS], sh_l[WARPS];
+    __shared__ float sh_o[WARPS][D];
+    const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
+    const int64_t bh = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
     grid_launch_dependents();
     grid_dependency_wait();
-    int64_t c0 = 0, pieces = 0;      // own pieces: of CTAs c0, c0 + 1, ...
+    if (bh >= static_cast<int64_t>(p.B) * p.Hq) return;   // with one warp per row only: whole warps
+    const int b = static_cast<int>(static_cast<uint32_t>(bh) / static_cast<uint32_t>(p.Hq));
+    const int h = static_cast<int>(bh) - b * p.Hq, hk = h / p.group, in_group = h - hk * p.group;
+    const int tile = in_group / nq, q = in_group - tile * nq;
+    const int W = p.Hkv * p.tiles, hw = hk * p.tiles + tile;
+    int c0 = 0, pieces = 0;          // own pieces: of CTAs c0, c0 + 1, ...
     bool complete = false;
     if (p.own) {
-        const int64_t units = p.before[b + 1] - p.before[b], total = p.before[p.B] * W;
-        const int64_t first = p.before[b] * W + hw * units;
-        const int64_t ctas = ctas_of(p, total);
-        c0 = holder(first, total, ctas);
-        pieces = holder(first + units - 1, total, ctas) - c0 + 1;
+        const int before = p.before[b], places = p.before[b + 1] - before, total = p.before[p.B] * W;
+        const int first = before * W + hw * places, ctas = ctas_of(p, total);
+        c0 = holder(first + kStart, total, ctas);
+        pieces = holder(first + places - 1, total, ctas) - c0 + 1;
         complete = pieces == 1 || p.whole;
         if (complete) pieces = 1;
         if (complete && p.prefix.splits == 0) return;
     }
-    const int64_t shared_row = p.prefix.splits == 0 ? 0 : hk * p.prefix.rows + b * p.group + in_group;
-    const int64_t shared_step = p.prefix.splits == 0 ? 0 : static_cast<int64_t>(p.Hkv) * p.prefix.rows;
-    const int64_t count = p.prefix.splits + pieces;
-    auto at = [&](int64_t i, const float2** ml, const float** o) {
-        if (i < p.prefix.splits) {
-            const int64_t r = i * shared_step + shared_row;
-            *ml = p.prefix.ml + r;
-            *o = p.prefix.o + r * D;
-            return;
-        }
-        i -= p.prefix.splits;
-        const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + b * W + hw : 2 * (c0 + i) + (i == 0 ? 1 : 0);
-        *ml = p.part_ml + slot * nq + q;
-        *o = p.part_o + (slot * nq + q) * D;
-    };
-    const float2* ml;
-    const float* src;
-    float mm = -INFINITY;
-    for (int64_t i = threadIdx.x; i < count; i += 128) {
-        at(i, &ml, &src);
-        mm = fmaxf(mm, ml->x);
-    }
-    mm = warp_max(mm);
-    if (lane == 0) red[warp] = mm;
-    __syncthreads();
-    mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float base = mm == -INFINITY ? 0.f : mm;
-    constexpr int N = D / 32;
-    float o[N], l = 0.f;
+    const int64_t shared_row = static_cast<int64_t>(hk) * p.prefix.rows + static_cast<int64_t>(b) * p.group + in_group, shared_step = static_cast<int64_t>(p.Hkv) * p.prefix.rows;
+    const int count = p.prefix.splits + pieces;
+    float m = kLowest, l = 0.f, o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = 0.f;
 #pragma unroll 4
-    for (int64_t i = warp; i < count; i += 4) {
-        at(i, &ml, &src);
-        const float2 x = *ml;
-        const float f = exp2_approx(x.x - base);
-        l += x.y * f;
-        if constexpr (N == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(src + lane * 4);
-            o[0] += y.x * f; o[1] += y.y * f; o[2] += y.z * f; o[3] += y.w * f;
+    for (int i = warp; i < count; i += WARPS) {
+        const float2* ml;
+        const float* src;
+        if (i < p.prefix.splits) {
+            const int64_t r = i * shared_step + shared_row;
+            ml = p.prefix.ml + r;
+            src = p.prefix.o + r * D;
         } else {
-            const float2 y = *reinterpret_cast<const float2*>(src + lane * 2);
-            o[0] += y.x * f; o[1] += y.y * f;
+            const int j = i - p.prefix.splits;
+            const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + static_cast<int64_t>(b) * W + hw : 2 * static_cast<int64_t>(c0 + j) + (j == 0 ? 1 : 0);
+            ml = p.part_ml + slot * nq + q;
+            src = p.part_o + (slot * nq + q) * D;
+        }
+        const float2 x = *ml;
+        float y[N];
+        if constexpr (N == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
+            y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(src + lane * 2);
+            y[0] = v.x; y[1] = v.y;
+        }
+        const float top = fmaxf(m, x.x), fa = exp2_approx(m - top), fb = exp2_approx(x.x - top);
+        m = top;
+        l = l * fa + x.y * fb;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[k] = o[k] * fa + y[k] * fb;
+    }
+    if constexpr (WARPS > 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) sh_o[warp][lane * N + i] = o[i];
+        if (lane == 0) {
+            sh_m[warp] = m;
+            sh_l[warp] = l;
+        }
+        __syncthreads();
+        if (warp != 0) return;
+        m = warp_max(lane < WARPS ? sh_m[lane] : kLowest);
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = exp2_approx(sh_m[w] - m);
+            l += sh_l[w] * f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] += sh_o[w][lane * N + i] * f;
         }
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * p.o_sh) + lane * (N / 2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sh_o[warp][lane * N + i] = o[i];
-    if (lane == 0) sh_l[warp] = l;
-    __syncthreads();
-    const float ll = (sh_l[0] + sh_l[1]) + (sh_l[2] + sh_l[3]);
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    for (int c = threadIdx.x * 2; c < D; c += 256) {
-        const float x = ((sh_o[0][c] + sh_o[1][c]) + (sh_o[2][c] + sh_o[3][c])) * inv, y = ((sh_o[0][c + 1] + sh_o[1][c + 1]) + (sh_o[2][c + 1] + sh_o[3][c + 1])) * inv;
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * p.o_sh + c) = Pair<T>::narrow(make_float2(x, y));
-    }
-    if (threadIdx.x == 0 && p.lse != nullptr) p.lse[b * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh] = ll == 0.f ? -INFINITY : (base + log2f(ll)) * 0.6931471805599453f;
+    for (int i = 0; i < N; i += 2) dst[i / 2] = Pair<T>::narrow(make_float2(o[i] * inv, o[i + 1] * inv));
+    if (lane == 0 && p.lse != nullptr) p.lse[b * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-template <typename T, bool QUANT, int D>
-cudaError_t launch_own(const CachedAttnParams& p, int nt, cudaStream_t stream) {
-    return nt == 1 ? launch_dependent(cached_attention_kernel<T, QUANT, D, 1>, static_cast<unsigned>(p.max_ctas), 128, 0, stream, p)
-                   : launch_dependent(cached_attention_kernel<T, QUANT, D, 2>, static_cast<unsigned>(p.max_ctas), 128, 0, stream, p);
+template <typename T, bool QUANT, int D, int NT>
+cudaError_t launch_own(const CachedAttnParams& p, cudaStream_t stream) {
+    const auto kernel = cached_attention_kernel<T, QUANT, D, NT>;
+    constexpr int smem = Ring<QUANT, D, NT>::kTotal;
+    if (cudaError_t e = tc_ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem); e != cudaSuccess) return e;
+    return launch_dependent(kernel, static_cast<unsigned>(p.max_ctas), 128, smem, stream, p);
 }
 template <typename T, int D>
 cudaError_t launch_attention(const CachedAttnParams& p, int nt, cudaStream_t stream) {
     if (p.own) {
-        const cudaError_t e = p.ks != nullptr ? launch_own<T, true, D>(p, nt, stream) : launch_own<T, false, D>(p, nt, stream);
+        cudaError_t e;
+        if (p.ks != nullptr) e = nt == 1 ? launch_own<T, true, D, 1>(p, stream) : launch_own<T, true, D, 2>(p, stream);
+        else e = nt == 1 ? launch_own<T, false, D, 1>(p, stream) : launch_own<T, false, D, 2>(p, stream);
         if (e != cudaSuccess) return e;
     }
     if (p.whole && p.own && p.prefix.splits == 0) return cudaSuccess;
-    return launch_dependent(cached_attention_join_kernel<T, D>, static_cast<unsigned>(static_cast<int64_t>(p.B) * p.Hq), 128, 0, stream, p, 8 * nt);
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq;
+    if (rows >= kWarpRows) return launch_dependent(cached_attention_join_kernel<T, D, 1>, static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, p, 8 * nt);
+    return launch_dependent(cached_attention_join_kernel<T, D, 16>, static_cast<unsigned>(rows), 512, 0, stream, p, 8 * nt);
 }
 
 // CTAs of a variant that an SM holds at once.
-template <typename T, bool QUANT, int D, int NT>
-int resident_of() {
-    static const int n = [] {
-        int v = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, cached_attention_kernel<T, QUANT, D, NT>, 128, 0) != cudaSuccess || v < 1) v = 1;
-        return v;
-    }();
-    return n;
-}
-template <typename T>
 int resident_ctas(int64_t D, bool quant, int nt) {
-    if (D == 128) return quant ? (nt == 1 ? resident_of<T, true, 128, 1>() : resident_of<T, true, 128, 2>())
-                               : (nt == 1 ? resident_of<T, false, 128, 1>() : resident_of<T, false, 128, 2>());
-    return quant ? (nt == 1 ? resident_of<T, true, 64, 1>() : resident_of<T, true, 64, 2>())
-                 : (nt == 1 ? resident_of<T, false, 64, 1>() : resident_of<T, false, 64, 2>());
+    if (D == 128) return quant ? (nt == 1 ? Ring<true, 128, 1>::kCtas : Ring<true, 128, 2>::kCtas) : (nt == 1 ? Ring<false, 128, 1>::kCtas : Ring<false, 128, 2>::kCtas);
+    return quant ? (nt == 1 ? Ring<true, 64, 1>::kCtas : Ring<true, 64, 2>::kCtas) : (nt == 1 ? Ring<false, 64, 1>::kCtas : Ring<false, 64, 2>::kCtas);
 }
 
 // What both entry points take, checked and gathered. `prefix_k` NULL: no shared rows.
@@ -666,8 +846,8 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     if (vq.numel == 0) return diopiSuccess;
     const int64_t group = Hq / Hkv;
     const int nt = group <= 8 ? 1 : 2;
-    const int64_t tiles = (group + 8 * nt - 1) / (8 * nt), segments = B * Hkv * tiles, most_units = segments * ((L + kUnit - 1) / kUnit);
-    B200_CHECK(most_units < (1ll << 40), "%s: too many keys", name);
+    const int64_t tiles = (group + 8 * nt - 1) / (8 * nt), segments = B * Hkv * tiles, most_places = segments * ((L + kUnit - 1) / kUnit + 1 + kStart);
+    B200_CHECK(segments < (1ll << 31) && most_places < (1ll << 31), "%s: too many keys", name);
     CachedAttnParams p = {};
     p.q = vq.data; p.out = vo.data;
     p.q_sb = vq.stride[0]; p.q_sh = vq.stride[1]; p.o_sb = vo.stride[0]; p.o_sh = vo.stride[1];
@@ -688,8 +868,8 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     p.whole = L <= kWholeKeys ? 1 : 0;
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
     const bool wide = vq.dtype == diopi_dtype_bfloat16;
-    const int64_t resident = static_cast<int64_t>(sm_count()) * (wide ? resident_ctas<bf16>(D, k_scale != nullptr, nt) : resident_ctas<fp16>(D, k_scale != nullptr, nt));
-    const int64_t wanted = p.whole ? segments : (most_units + kMinUnits - 1) / kMinUnits;
+    const int64_t resident = static_cast<int64_t>(sm_count()) * resident_ctas(D, k_scale != nullptr, nt);
+    const int64_t wanted = p.whole ? segments : (most_places + kMinPlaces - 1) / kMinPlaces;
     p.max_ctas = static_cast<int>(wanted < resident ? (wanted < 1 ? 1 : wanted) : resident);
     cudaStream_t stream = stream_of(ctx);
     if (P > 0) {
@@ -699,12 +879,12 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     const bool join = !p.whole || p.prefix.splits > 0;
     if (p.own && join) {
         const int64_t slots = (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + (P > 0 ? segments : 0), rows = slots * 8 * nt;
-        const int64_t head = ((B + 1) * 8 + 255) / 256 * 256;
+        const int64_t head = ((B + 1) * 4 + 255) / 256 * 256;
         diopiTensorHandle_t ws = nullptr;
         void* ptr = nullptr;
         B200_CHECK(diopiRequireBuffer(ctx, &ws, head + rows * (D * 4 + 8), diopi_device) == diopiSuccess && ws != nullptr, "%s: workspace allocation failed", name);
         B200_CHECK(diopiGetTensorData(ws, &ptr) == diopiSuccess && ptr != nullptr, "%s: workspace has no data pointer", name);
-        p.before = static_cast<int64_t*>(ptr);
+        p.before = static_cast<int*>(ptr);
         p.part_o = reinterpret_cast<float*>(static_cast<char*>(ptr) + head);
         p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * D);
     }
