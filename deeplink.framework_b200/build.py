@@ -5,6 +5,7 @@
     lib/libdiopirt_minihost.so   a small DIOPI host (the diopirt callbacks over plain tensor structs)
     lib/libdiopi_impl.so         the DIOPI operator library: hand-written sm_100a kernels
     lib/libtorch_dipu_b200.so             hot-path aten ops on the PrivateUse1 key ("dipu"), each wrapper calling ::diopiXxx
+    lib/dipu_b200_call.<abi>.so           DIOPI calls from Python with stack-allocated tensor handles, as a Python extension module
     lib/dipu_b200_c10d.<abi>.so           the c10d backend "dicl" (torch.distributed on dipu tensors) as a Python extension module
     lib/libdipu_vendor_b200_torchabi.so   the vendor contract with DIPU's exact C++ signatures (namespace dipu::devapis, torch
                                  types in the arguments): thin wrappers over the C-ABI runtime, built when torch's headers are present
@@ -103,6 +104,16 @@ def _build_torch_c10d(verbose):
                             extra_cflags=["-DTORCH_EXTENSION_NAME=dipu_b200_c10d", "-I", py_inc], extra_link=["-ltorch_python", "-ltorch"])
 
 
+def _build_torch_call(verbose):
+    """csrc/torch_call/*.cpp: the Python extension module that calls DIOPI functions with stack-allocated tensor handles."""
+    import sysconfig
+    suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+    py_inc = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(py_inc, "Python.h")):
+        return None
+    return _build_torch_lib("torch_call", "dipu_b200_call" + suffix, [], verbose, extra_cflags=["-I", py_inc, "-I", CSRC], extra_link=["-ltorch_python", "-ltorch"])
+
+
 def _build_torch_lib(sub, out_name, link_libs, verbose, extra_cflags=(), extra_link=()):
     try:
         import torch
@@ -168,6 +179,9 @@ def build(verbose=False):
         c10d = _build_torch_c10d(verbose)
         if c10d:
             built.append(c10d)
+    call = _build_torch_call(verbose)
+    if call:
+        built.append(call)
     return built
 
 

@@ -6,6 +6,9 @@ device, exactly the metadata DIPU's diopirt callbacks expose. Every diopiXxx fun
 a non-zero return code raises DiopiError carrying diopiGetLastErrorString().
 """
 import ctypes
+import glob
+import importlib.util
+import os
 
 import torch
 
@@ -13,6 +16,20 @@ from . import _native
 
 _lib = _native.diopi
 _host = _native.host
+
+
+def _load_call():
+    """The extension module that fills the tensor handles in C++ (built when torch's and Python's headers are present)."""
+    paths = glob.glob(os.path.join(_native.LIB_DIR, "dipu_b200_call*.so"))
+    if not paths:
+        return None
+    spec = importlib.util.spec_from_file_location("dipu_b200_call", paths[0])
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+_call = _load_call()
 
 # ---- enums (include/diopi/diopirt.h) -------------------------------------------------------------------------
 diopi_host, diopi_device = 0, 1
@@ -198,6 +215,20 @@ def _bind(name):
             argtypes.append(_CTYPES[c])
     fn.argtypes = argtypes
     fn.restype = ctypes.c_int
+
+    if _call is not None and set(sig) <= set("Ttsirdb"):
+        bound = _call.bind(ctypes.cast(fn, ctypes.c_void_p).value, sig, DiopiError)
+
+        def fast(ctx, *args):
+            if len(args) != len(sig):
+                raise TypeError("%s expects %d arguments after ctx, got %d" % (name, len(sig), len(args)))
+            rc = bound(ctx.ptr, *args)
+            if rc != 0:
+                raise DiopiError("%s failed with code %d: %s" % (name, rc, last_error()))
+            return rc
+
+        fast.__name__ = name
+        return fast
 
     def call(ctx, *args):
         if len(args) != len(sig):

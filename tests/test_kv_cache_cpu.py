@@ -8,23 +8,14 @@ import torch
 BF, FP, F32, I8, I64 = torch.bfloat16, torch.float16, torch.float32, torch.int8, torch.int64
 
 
-@pytest.fixture()
-def on_device(diopi, monkeypatch):
-    """diopi.handle() for host tensors whose handles claim to be device tensors (unless they are marked as the host's)."""
-    made = []
-
-    def handle(t):
-        nd = t.dim()
-        shape, stride = ((ctypes.c_int64 * max(nd, 1))(*v) for v in (t.shape, t.stride()))
-        h = type("H", (), {})()
-        h.ptr = diopi._host.minihostMakeTensor(ctypes.c_void_p(t.data_ptr()), nd, shape, stride, diopi.DTYPE[t.dtype], 0 if getattr(t, "on_host", False) else 1, 0)
-        made.append(h.ptr)
-        return h
-
-    monkeypatch.setattr(diopi, "handle", handle)
-    yield diopi
-    for p in made:
-        diopi._host.minihostFreeTensor(p)
+def _handle(diopi, t):
+    """A handle for a host tensor that claims to be a device tensor (unless it is marked as the host's)."""
+    h = diopi.Handle(t)
+    if not getattr(t, "on_host", False):
+        diopi._host.minihostFreeTensor(ctypes.c_void_p(h.ptr))
+        shape, stride = ((ctypes.c_int64 * t.dim())(*v) for v in (t.shape, t.stride()))
+        h.ptr = diopi._host.minihostMakeTensor(ctypes.c_void_p(t.data_ptr()), t.dim(), shape, stride, diopi.DTYPE[t.dtype], 1, 0)
+    return h
 
 
 def _aligned(shape, dtype):
@@ -77,8 +68,9 @@ def _off(t):
 
 def _refused(diopi, name, args, match):
     ctx = diopi.Context()
+    handles = [_handle(diopi, a) if isinstance(a, torch.Tensor) else a for a in args.values()]
     with pytest.raises(diopi.DiopiError, match=match):
-        getattr(diopi, name)(ctx, *args.values())
+        getattr(diopi, name)(ctx, *handles)
 
 
 _WRITE = [
@@ -110,8 +102,8 @@ _WRITE = [
 
 
 @pytest.mark.parametrize("change,match", _WRITE)
-def test_write_refuses(on_device, change, match):
-    _refused(on_device, "diopiB200RopeQuantAppendKV", {**_write_args(), **change}, match)
+def test_write_refuses(diopi, change, match):
+    _refused(diopi, "diopiB200RopeQuantAppendKV", {**_write_args(), **change}, match)
 
 
 @pytest.mark.parametrize("change,match", [
@@ -122,8 +114,8 @@ def test_write_refuses(on_device, change, match):
     ({"k_out": _aligned((1, S, HKV, D), BF).expand(B, S, HKV, D)}, "pitches"),
     ({"positions": _aligned((2 * B,), I64)[::2]}, "positions must be"),
 ])
-def test_read_back_refuses(on_device, change, match):
-    _refused(on_device, "diopiB200DequantKV", {**_dequant_args(), **change}, match)
+def test_read_back_refuses(diopi, change, match):
+    _refused(diopi, "diopiB200DequantKV", {**_dequant_args(), **change}, match)
 
 
 _ATTENTION = [
@@ -152,14 +144,14 @@ _ATTENTION = [
 
 @pytest.mark.parametrize("entry", ["diopiB200CachedAttention", "diopiB200SharedPrefixAttention"])
 @pytest.mark.parametrize("change,match", _ATTENTION)
-def test_attention_refuses(on_device, entry, change, match):
+def test_attention_refuses(diopi, entry, change, match):
     args = _attention_args() if entry == "diopiB200CachedAttention" else _prefix_args()
-    _refused(on_device, entry, {**args, **change}, match)
+    _refused(diopi, entry, {**args, **change}, match)
 
 
-def test_attention_refuses_out_that_is_q(on_device):
+def test_attention_refuses_out_that_is_q(diopi):
     a = _attention_args()
-    _refused(on_device, "diopiB200CachedAttention", {**a, "out": a["q"]}, "out must not be q")
+    _refused(diopi, "diopiB200CachedAttention", {**a, "out": a["q"]}, "out must not be q")
 
 
 @pytest.mark.parametrize("change,match", [
@@ -168,8 +160,8 @@ def test_attention_refuses_out_that_is_q(on_device):
     ({"v_cache": _aligned((B, HKV, L + 1, D), BF)}, "same shape"),
     ({"k_cache": _aligned((B, HKV, L, D + 4), BF)[..., :D]}, "pitches"),
 ])
-def test_attention_over_the_models_type_refuses(on_device, change, match):
-    _refused(on_device, "diopiB200CachedAttention", {**_attention_args(False), **change}, match)
+def test_attention_over_the_models_type_refuses(diopi, change, match):
+    _refused(diopi, "diopiB200CachedAttention", {**_attention_args(False), **change}, match)
 
 
 @pytest.mark.parametrize("change,match", [
@@ -182,5 +174,26 @@ def test_attention_over_the_models_type_refuses(on_device, change, match):
     ({"prefix_v": _host(_aligned((P, HKV, D), BF))}, "device"),
     ({"prefix_v": _aligned((P * HKV * 3 * D,), BF).as_strided((P, HKV, D), (2 * D + 24, D, 1))}, "multiple of the other"),
 ])
-def test_prefix_refuses(on_device, change, match):
-    _refused(on_device, "diopiB200SharedPrefixAttention", {**_prefix_args(), **change}, match)
+def test_prefix_refuses(diopi, change, match):
+    _refused(diopi, "diopiB200SharedPrefixAttention", {**_prefix_args(), **change}, match)
+
+
+def test_binding_arguments(diopi):
+    """The binding passes what it is given, and raises for what it cannot pass, with handles and with tensors alike."""
+    ctx = diopi.Context()
+    a = _attention_args()
+    with pytest.raises(diopi.DiopiError, match="must live on the device"):   # host tensors, described as such
+        diopi.diopiB200CachedAttention(ctx, *a.values())
+    with pytest.raises(TypeError, match="expects 9 arguments"):
+        diopi.diopiB200CachedAttention(ctx, *list(a.values())[:-1])
+    with pytest.raises(diopi.DiopiError, match="no diopi counterpart"):
+        diopi.diopiB200CachedAttention(ctx, *{**a, "q": torch.zeros(1, dtype=torch.complex64)}.values())
+    with pytest.raises(diopi.DiopiError, match="tensor handle is NULL"):
+        diopi.diopiB200CachedAttention(ctx, *{**a, "q": None}.values())
+    with pytest.raises((TypeError, ValueError)):
+        diopi.diopiB200CachedAttention(ctx, *{**a, "scale": "x"}.values())
+    with pytest.raises(AttributeError):
+        diopi.diopiB200CachedAttention(ctx, *{**a, "q": 3}.values())
+    big = [_handle(diopi, x) if isinstance(x, torch.Tensor) else x for x in a.values()]
+    with pytest.raises(diopi.DiopiError, match="scale must be positive, got -0.25"):
+        diopi.diopiB200CachedAttention(ctx, *big[:-1], -0.25)
