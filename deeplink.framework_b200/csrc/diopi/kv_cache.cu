@@ -16,124 +16,216 @@
 namespace b200 {
 namespace {
 
+constexpr int kPasses = 3;         // rows a thread of the writer has in flight
+constexpr int64_t kManyRows = 32768;   // from so many rows on the writer's threads take 16 values instead of 8
+constexpr int kTokens = 2;         // tokens a CTA of the read-back takes
+
 struct AppendParams {
     const void* qkv;
     int64_t x_sb, x_ss;            // element pitches between sequences and tokens
     void* q_out;
     int64_t q_sb, q_ss, q_sh;
-    int8_t* k_cache;
-    int8_t* v_cache;
-    float* k_scale;
-    float* v_scale;
-    int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;      // cache pitches (bytes = elements)
-    int64_t ks_sb, ks_sh, vs_sb, vs_sh;              // scale pitches; slots are neighbours
+    int8_t* cache[2];              // k, v
+    float* scale[2];
+    int64_t c_sb[2], c_sh[2], c_sl[2];   // cache pitches (bytes = elements)
+    int64_t s_sb[2], s_sh[2];            // scale pitches; slots are neighbours
     const float* cos_t;
     const float* sin_t;            // [table_rows, rot / 2]
     const int64_t* positions;
-    int64_t S, L, table_rows, items;
-    int Hq, Hkv, rot;
+    int64_t L, table_rows;
+    int S, Hq, Hkv, rot;
+    int per_cta;                   // passes a CTA takes, at most kPasses
 };
 
-// One thread of a row: 8 values in two groups of four. Half-split layout: values 4c .. 4c+3 of the first half of the rotated part
-// and their partners; the part behind it, interleaved pairs and v rows: 8 neighbours.
-template <typename T, int D, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rope_quant_append_kernel(const AppendParams p) {
-    constexpr int LANES = D / 8;   // threads per row
-    const int64_t item = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
-    const int c = threadIdx.x % LANES;
-    const int heads = p.Hq + 2 * p.Hkv;
-    const bool live = item < p.items;
-    grid_launch_dependents();   // the attention that follows may set itself up meanwhile
-    const int64_t token = live ? item / heads : 0;
-    const int h = live ? static_cast<int>(item - token * heads) : 0;
-    const int64_t b = token / p.S, s = token - b * p.S;
-    const int64_t start = live ? p.positions[b] : -1;
-    const int64_t slot = start + s;
-    const bool write = start >= 0 && start < p.L && slot < p.L && (p.rot == 0 || slot < p.table_rows);
+// Largest of three magnitudes; a NaN among them is the result.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
+__device__ __forceinline__ float max_abs8(float2 a, float2 b, float2 c, float2 d) {
+    return max_abs(max_abs3(max_abs3(a.x, a.y, b.x), b.y, c.x), max_abs3(c.y, d.x, d.y));
+}
 
-    const bool rotate = h < p.Hq + p.Hkv && c < p.rot / 8;
-    const int lo = (!INTERLEAVED && rotate) ? 4 * c : 8 * c;
-    const int hi = (!INTERLEAVED && rotate) ? p.rot / 2 + 4 * c : 8 * c + 4;
-    float2 y[4];   // values lo, lo+1 | lo+2, lo+3 | hi, hi+1 | hi+2, hi+3
+// The codes of 8 values, four to a word. amax: the row's largest magnitude, NaN if it holds one.
+__device__ __forceinline__ uint2 quantise(const float2 (&y)[4], float amax, float scale) {
+    uint32_t code[8];
+    if (amax > 1e-30f && amax < INFINITY) {
+        // y * (127 / max|y|) + 1.5 * 2^23, rounded once to nearest even: the low byte of the sum is the code. Where the product is
+        // within 2^-12 of a tie (it is within 127 * 2^-20 of the quotient) the quotient decides: a row's values are few bits long,
+        // so half of the largest one, code 63.5, is no rare value.
+        const float r = __fdividef(127.f, amax);
+        const float2 rr = make_float2(r, r), magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-1.f, -1.f);
+        float2 d[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = make_float2(0.f, 0.f);
-    if (write) {
-        const T* src = static_cast<const T*>(p.qkv) + b * p.x_sb + s * p.x_ss + static_cast<int64_t>(h) * D;
-        const uint2 wa = __ldcs(reinterpret_cast<const uint2*>(src + lo)), wb = __ldcs(reinterpret_cast<const uint2*>(src + hi));
-        y[0] = Pair<T>::widen(wa.x); y[1] = Pair<T>::widen(wa.y);
-        y[2] = Pair<T>::widen(wb.x); y[3] = Pair<T>::widen(wb.y);
-        if (rotate) {
-            const float4 cs = *reinterpret_cast<const float4*>(p.cos_t + slot * (p.rot / 2) + 4 * c);
-            const float4 sn = *reinterpret_cast<const float4*>(p.sin_t + slot * (p.rot / 2) + 4 * c);
-            if (INTERLEAVED) {
-                const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+        for (int i = 0; i < 4; ++i) {
+            const float2 s = fma2(y[i], rr, magic);
+            code[2 * i] = __float_as_uint(s.x);
+            code[2 * i + 1] = __float_as_uint(s.y);
+            d[i] = fma2(y[i], rr, fma2(s, minus, magic));   // the product minus its code
+        }
+        if (max_abs8(d[0], d[1], d[2], d[3]) > 0.5f - 0x1p-12f) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = make_float2(fmaf(y[i].y, -ss[i], y[i].x * cc[i]), fmaf(y[i].x, ss[i], y[i].y * cc[i]));
-            } else {
-                const float2 cc[2] = {make_float2(cs.x, cs.y), make_float2(cs.z, cs.w)}, ss[2] = {make_float2(sn.x, sn.y), make_float2(sn.z, sn.w)};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float2 a = y[i], bb = y[2 + i];
-                    y[i] = fma2(bb, make_float2(-ss[i].x, -ss[i].y), mul2(a, cc[i]));
-                    y[2 + i] = fma2(a, ss[i], mul2(bb, cc[i]));
+            for (int i = 0; i < 8; ++i) {
+                const float di = (i & 1) ? d[i >> 1].y : d[i >> 1].x;
+                if (fabsf(di) > 0.5f - 0x1p-12f) {
+                    // The border h = k + 1/2 next to it, and y - h scale, exact (the difference is small and the product 32 bits
+                    // long): the fp32 quotient is h itself up to half a unit in its last place, and then goes to the even side.
+                    const float v = (i & 1) ? y[i >> 1].y : y[i >> 1].x;
+                    const float k = __uint_as_float(code[i]) - 12582912.f, h = k + copysignf(0.5f, di), rest = fmaf(-h, scale, v);
+                    const float half_unit = __uint_as_float((__float_as_uint(h) & 0x7f800000u) - (24u << 23));
+                    const float to = fabsf(rest) <= half_unit * scale ? rintf(h) : (rest > 0.f ? ceilf(h) : floorf(h));
+                    code[i] = __float_as_uint(to + 12582912.f);
                 }
             }
         }
-    }
-    // Largest magnitude of the row. Compared as bit patterns: infinities and NaN are the largest, and none gets lost.
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(__float_as_uint(y[i].x) & 0x7fffffffu, __float_as_uint(y[i].y) & 0x7fffffffu));
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!write) return;
-    if (h < p.Hq) {
-        T* dst = static_cast<T*>(p.q_out) + b * p.q_sb + s * p.q_ss + static_cast<int64_t>(h) * p.q_sh;
-        *reinterpret_cast<uint2*>(dst + lo) = make_uint2(Pair<T>::narrow(y[0]), Pair<T>::narrow(y[1]));
-        *reinterpret_cast<uint2*>(dst + hi) = make_uint2(Pair<T>::narrow(y[2]), Pair<T>::narrow(y[3]));
-        return;
-    }
-    const bool is_k = h < p.Hq + p.Hkv;
-    const int64_t hk = is_k ? h - p.Hq : h - p.Hq - p.Hkv;
-    const float amax = __uint_as_float(top);
-    const bool finite = top < 0x7f800000u;
-    const float scale = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
-    uint32_t code[8];
-    if (amax > 1e-30f && finite) {
-        // y * (127 / max|y|) + 1.5 * 2^23, rounded once to nearest even: the low byte of the sum is the code. Where the product is
-        // within 2^-12 of a tie the quotient itself decides (the product is within 127 * 2^-22 of it): a row's values are few
-        // bits long, so half of the largest one, code 63.5, is no rare value.
-        const float r = 127.f / amax;
-        float off = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = (i & 1) ? y[i >> 1].y : y[i >> 1].x, s = fmaf(x, r, 12582912.f);
-            code[i] = __float_as_uint(s);
-            off = fmaxf(off, fabsf(fmaf(x, r, 12582912.f - s)));
-        }
-        if (off > 0.5f - 0x1p-12f) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) code[i] = static_cast<uint32_t>(__float2int_rn(((i & 1) ? y[i >> 1].y : y[i >> 1].x) / scale));
-        }
     } else {
         // rows so small that 127 / max|y| may overflow, rows of zeros (also those whose scale underflows to zero), rows that are not finite
-        const bool zero = !finite || scale == 0.f;
+        const bool zero = !(amax < INFINITY) || scale == 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            code[2 * i] = zero ? 0u : static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(y[i].x / scale, -127.f), 127.f)));
-            code[2 * i + 1] = zero ? 0u : static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(y[i].y / scale, -127.f), 127.f)));
+        for (int i = 0; i < 8; ++i) {
+            const float x = (i & 1) ? y[i >> 1].y : y[i >> 1].x;
+            code[i] = zero ? 0u : static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x / scale, -127.f), 127.f)));
         }
     }
-    uint32_t w[2];
+    return make_uint2(__byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410));
+}
+
+// H consecutive 2-byte values of a row, H = 4 or 8.
+template <int H>
+struct Half {
+    uint32_t w[H / 2];
+    template <typename T>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (H == 8) {
+            const uint4 v = ld16_stream_raw(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+            w[0] = v.x; w[1] = v.y;
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (H == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    }
+};
+
+// A thread takes 2 H values of a row in two groups: values H c .. H c + H - 1 of the first half of the rotated part and their
+// partners in the half-split layout, neighbours in the part behind it, for interleaved pairs and for values. The rows of a token come
+// in passes of as many rows as the CTA has groups of D / 2H threads, first those of q, then those of k and v; a CTA takes up to
+// kPasses of them and has their loads in flight together. Whether a pass is q or not is the same for the whole CTA, and a thread's
+// angles serve all its rows. Bound by memory: 2 D bytes in per row, 2 D (q) or D + 4 out. H = 8 halves the work around a row
+// ([16384 tokens, 32 + 2 x 32 heads of 128] 200 -> 155 us), H = 4 is the shorter chain (64 tokens: 5.3 -> 4.3 us).
+template <typename T, int D, bool INTERLEAVED, int H>
+__global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendParams p) {
+    constexpr int LANES = D / (2 * H), ROWS = 256 / LANES;
+    const int c = threadIdx.x % LANES, r = threadIdx.x / LANES;
+    grid_launch_dependents();   // the attention that follows may set itself up meanwhile
+    const int b = blockIdx.x / static_cast<unsigned>(p.S), s = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * p.S);
+    const int64_t start = p.positions[b];
+    const int q_passes = (p.Hq + ROWS - 1) / ROWS, first = blockIdx.y * p.per_cta;
+    const bool turns = c < p.rot / (2 * H);
+    const int half_lo = !INTERLEAVED && turns ? H * c : 2 * H * c, half_hi = !INTERLEAVED && turns ? p.rot / 2 + H * c : 2 * H * c + H;
+    const T* src = static_cast<const T*>(p.qkv) + b * p.x_sb + s * p.x_ss;
+    Half<H> wa[kPasses], wb[kPasses];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040), __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410);
-    int8_t* dst = is_k ? p.k_cache + b * p.k_sb + hk * p.k_sh + slot * p.k_sl : p.v_cache + b * p.v_sb + hk * p.v_sh + slot * p.v_sl;
-    *reinterpret_cast<uint32_t*>(dst + lo) = w[0];
-    *reinterpret_cast<uint32_t*>(dst + hi) = w[1];
-    if (c == 0) {
-        float* sc = is_k ? p.k_scale + b * p.ks_sb + hk * p.ks_sh + slot : p.v_scale + b * p.vs_sb + hk * p.vs_sh + slot;
-        *sc = scale;
+    for (int u = 0; u < kPasses; ++u) {
+        const int pass = first + u;
+        const int h = pass < q_passes ? pass * ROWS + r : p.Hq + (pass - q_passes) * ROWS + r;
+        wa[u] = wb[u] = Half<H>{};
+        if (u < p.per_cta && h < (pass < q_passes ? p.Hq : p.Hq + 2 * p.Hkv)) {
+            const bool is_v = h >= p.Hq + p.Hkv;
+            wa[u].load(src + h * D + (is_v ? 2 * H * c : half_lo));
+            wb[u].load(src + h * D + (is_v ? 2 * H * c + H : half_hi));
+        }
+    }
+    if (start < 0 || start >= p.L) return;
+    const int64_t slot = start + s;
+    if (slot >= p.L || (p.rot != 0 && slot >= p.table_rows)) return;
+    float2 cs[H / 2], sn[H / 2];
+#pragma unroll
+    for (int i = 0; i < H / 4; ++i) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (turns) {
+            x = *reinterpret_cast<const float4*>(p.cos_t + slot * (p.rot / 2) + H * c + 4 * i);
+            y = *reinterpret_cast<const float4*>(p.sin_t + slot * (p.rot / 2) + H * c + 4 * i);
+        }
+        cs[2 * i] = make_float2(x.x, x.y); cs[2 * i + 1] = make_float2(x.z, x.w);
+        sn[2 * i] = make_float2(y.x, y.y); sn[2 * i + 1] = make_float2(y.z, y.w);
+    }
+    T* const q_dst = static_cast<T*>(p.q_out) + b * p.q_sb + s * p.q_ss;
+    int8_t* const k_dst = p.cache[0] + b * p.c_sb[0] + slot * p.c_sl[0];
+    int8_t* const v_dst = p.cache[1] + b * p.c_sb[1] + slot * p.c_sl[1];
+    float* const k_scale = p.scale[0] + b * p.s_sb[0] + slot;
+    float* const v_scale = p.scale[1] + b * p.s_sb[1] + slot;
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+        const int pass = first + u;
+        if (u >= p.per_cta || (pass >= q_passes && (pass - q_passes) * ROWS >= 2 * p.Hkv)) return;
+        const bool is_q = pass < q_passes;
+        const int h = (is_q ? pass : pass - q_passes) * ROWS + r;
+        const bool is_v = !is_q && h >= p.Hkv;
+        float2 y[H];   // the first group's pairs of neighbours, then the second's
+#pragma unroll
+        for (int i = 0; i < H / 2; ++i) {
+            y[i] = Pair<T>::widen(wa[u].w[i]);
+            y[H / 2 + i] = Pair<T>::widen(wb[u].w[i]);
+        }
+        if (turns && !is_v) {
+#pragma unroll
+            for (int i = 0; i < H / 2; ++i) {
+                if (INTERLEAVED) {
+                    const float2 a = y[2 * i], bb = y[2 * i + 1];
+                    y[2 * i] = make_float2(fmaf(a.y, -sn[i].x, a.x * cs[i].x), fmaf(a.x, sn[i].x, a.y * cs[i].x));
+                    y[2 * i + 1] = make_float2(fmaf(bb.y, -sn[i].y, bb.x * cs[i].y), fmaf(bb.x, sn[i].y, bb.y * cs[i].y));
+                } else {
+                    const float2 a = y[i], bb = y[H / 2 + i];
+                    y[i] = fma2(bb, make_float2(-sn[i].x, -sn[i].y), mul2(a, cs[i]));
+                    y[H / 2 + i] = fma2(a, sn[i], mul2(bb, cs[i]));
+                }
+            }
+        }
+        if (is_q) {
+            if (h < p.Hq) {
+                Half<H> lo, hi;
+#pragma unroll
+                for (int i = 0; i < H / 2; ++i) {
+                    lo.w[i] = Pair<T>::narrow(y[i]);
+                    hi.w[i] = Pair<T>::narrow(y[H / 2 + i]);
+                }
+                T* dst = q_dst + h * p.q_sh;
+                lo.store(dst + half_lo);
+                hi.store(dst + half_hi);
+            }
+        } else {
+            float amax = max_abs8(y[0], y[1], y[2], y[3]);
+            if constexpr (H == 8) amax = max_abs(amax, max_abs8(y[4], y[5], y[6], y[7]));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) amax = max_abs(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            if (h < 2 * p.Hkv) {
+                const float scale = amax < INFINITY ? amax / 127.f : __uint_as_float(0x7fc00000u);
+                const int hk = is_v ? h - p.Hkv : h;
+                int8_t* dst = (is_v ? v_dst : k_dst) + hk * (is_v ? p.c_sh[1] : p.c_sh[0]);
+                int8_t *lo = dst + (is_v ? 2 * H * c : half_lo), *hi = dst + (is_v ? 2 * H * c + H : half_hi);
+                if constexpr (H == 8) {
+                    *reinterpret_cast<uint2*>(lo) = quantise({y[0], y[1], y[2], y[3]}, amax, scale);
+                    *reinterpret_cast<uint2*>(hi) = quantise({y[4], y[5], y[6], y[7]}, amax, scale);
+                } else {
+                    const uint2 w = quantise({y[0], y[1], y[2], y[3]}, amax, scale);
+                    *reinterpret_cast<uint32_t*>(lo) = w.x;
+                    *reinterpret_cast<uint32_t*>(hi) = w.y;
+                }
+                if (c == 0) *((is_v ? v_scale : k_scale) + hk * (is_v ? p.s_sh[1] : p.s_sh[0])) = scale;
+            }
+        }
     }
 }
 
@@ -143,35 +235,58 @@ struct DequantParams {
     void* out[2];
     int64_t c_sb[2], c_sh[2], c_sl[2], s_sb[2], s_sh[2], o_sb[2], o_ss[2], o_sh[2];
     const int64_t* positions;      // optional
-    int64_t S, L, items;
-    int Hkv;
+    int64_t L;
+    int S, chunks, Hkv;            // chunks of kTokens tokens per sequence
 };
 
+// D / 16 threads take a row, 16 values each: a CTA takes 256 / (D / 16) heads of kTokens tokens, of k and of v, with all loads in
+// flight. A code becomes fp32 as the low byte of 2^23 + 128 + code, exactly, and then one product is rounded.
+// Bound by memory: D + 4 bytes in, 2 D out.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
-    constexpr int LANES = D / 8;
-    const int which = blockIdx.y;  // 0: k, 1: v
-    const int64_t item = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
-    if (item >= p.items) return;
-    const int c = threadIdx.x % LANES;
-    const int64_t token = item / p.Hkv;
-    const int64_t h = item - token * p.Hkv;
-    const int64_t b = token / p.S, s = token - b * p.S;
+    constexpr int LANES = D / 16, ROWS = 256 / LANES;
+    const int c = threadIdx.x % LANES, h = blockIdx.y * ROWS + threadIdx.x / LANES;
+    const int b = blockIdx.x / static_cast<unsigned>(p.chunks), s0 = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * p.chunks) * kTokens;
     const int64_t start = p.positions != nullptr ? p.positions[b] : 0;
-    if (start < 0 || start >= p.L || start + s >= p.L) return;
-    const int64_t slot = start + s;
-    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p.cache[which] + b * p.c_sb[which] + h * p.c_sh[which] + slot * p.c_sl[which] + 8 * c));
-    const float scale = p.scale[which][b * p.s_sb[which] + h * p.s_sh[which] + slot];
-    const uint32_t words[2] = {w.x, w.y};
-    uint32_t o[4];
+    if (h >= p.Hkv || start < 0 || start >= p.L || start + s0 >= p.L) return;
+    const int64_t slot = start + s0;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(min(kTokens, p.S - s0)), p.L - slot));
+    uint4 v[2][kTokens];
+    float f[2][kTokens];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t u = words[i >> 1] >> ((i & 1) * 16);
-        const float2 v = make_float2(static_cast<float>(static_cast<int8_t>(u & 0xff)), static_cast<float>(static_cast<int8_t>((u >> 8) & 0xff)));
-        o[i] = Pair<T>::narrow(mul2(v, make_float2(scale, scale)));
+    for (int w = 0; w < 2; ++w) {
+        const int8_t* src = p.cache[w] + b * p.c_sb[w] + h * p.c_sh[w] + slot * p.c_sl[w] + 16 * c;
+        const float* scales = p.scale[w] + b * p.s_sb[w] + h * p.s_sh[w] + slot;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+            if (t < tokens) {
+                v[w][t] = ld16_stream_raw(src + t * p.c_sl[w]);
+                f[w][t] = scales[t];
+            }
+        }
     }
-    T* dst = static_cast<T*>(p.out[which]) + b * p.o_sb[which] + s * p.o_ss[which] + h * p.o_sh[which] + 8 * c;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        T* out = static_cast<T*>(p.out[w]) + b * p.o_sb[w] + s0 * p.o_ss[w] + h * p.o_sh[w] + 16 * c;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+            if (t < tokens) {
+                uint32_t o[8];
+                const float2 ff = make_float2(f[w][t], f[w][t]), bias = make_float2(-8388736.f, -8388736.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t x = word(v[w][t], i) ^ 0x80808080u;
+                    const float2 lo = make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7441)));
+                    const float2 hi = make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7443)));
+                    o[2 * i] = Pair<T>::narrow(mul2(add2(lo, bias), ff));
+                    o[2 * i + 1] = Pair<T>::narrow(mul2(add2(hi, bias), ff));
+                }
+                T* dst = out + t * p.o_ss[w];
+                *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(dst + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+        }
+    }
 }
 
 bool model_type(diopiDtype_t t) { return t == diopi_dtype_bfloat16 || t == diopi_dtype_float16; }
@@ -250,35 +365,45 @@ diopiError_t diopiB200RopeQuantAppendKV(diopiContextHandle_t ctx, diopiTensorHan
                    "%s: cos / sin must be dense 16-byte aligned float32 tables [positions, rotated / 2] on the device", name);
         table_rows = vc.shape[0];
         rot = 2 * vc.shape[1];
-        B200_CHECK(rot <= D && rot % 8 == 0, "%s: the rotated part (%lld) must be a multiple of 8 and at most the head dim", name, (long long)rot);
+        B200_CHECK(rot <= D && rot % 16 == 0, "%s: the rotated part (%lld) must be a multiple of 16 and at most the head dim", name, (long long)rot);
     }
     if (vx.numel == 0 || L == 0) return diopiSuccess;
+    B200_CHECK(B * S < 0x7fffffffLL && Hq + 2 * Hkv < 65536, "%s: too many tokens or heads", name);
     AppendParams p = {};
     p.qkv = vx.data; p.x_sb = vx.stride[0]; p.x_ss = tokens ? vx.stride[1] : 0;
     if (q_out) {
         p.q_out = vq.data; p.q_sb = vq.stride[0]; p.q_ss = tokens ? vq.stride[1] : 0; p.q_sh = vq.stride[vq.ndim - 2];
     }
-    p.k_cache = static_cast<int8_t*>(vk.data); p.v_cache = static_cast<int8_t*>(vv.data);
-    p.k_scale = static_cast<float*>(vks.data); p.v_scale = static_cast<float*>(vvs.data);
-    p.k_sb = vk.stride[0]; p.k_sh = vk.stride[1]; p.k_sl = vk.stride[2];
-    p.v_sb = vv.stride[0]; p.v_sh = vv.stride[1]; p.v_sl = vv.stride[2];
-    p.ks_sb = vks.stride[0]; p.ks_sh = vks.stride[1]; p.vs_sb = vvs.stride[0]; p.vs_sh = vvs.stride[1];
+    const TensorView* caches[2] = {&vk, &vv};
+    const TensorView* scales[2] = {&vks, &vvs};
+    for (int i = 0; i < 2; ++i) {
+        p.cache[i] = static_cast<int8_t*>(caches[i]->data); p.scale[i] = static_cast<float*>(scales[i]->data);
+        p.c_sb[i] = caches[i]->stride[0]; p.c_sh[i] = caches[i]->stride[1]; p.c_sl[i] = caches[i]->stride[2];
+        p.s_sb[i] = scales[i]->stride[0]; p.s_sh[i] = scales[i]->stride[1];
+    }
     if (cos) {
         p.cos_t = static_cast<const float*>(vc.data); p.sin_t = static_cast<const float*>(vsn.data);
     }
     p.positions = static_cast<const int64_t*>(vp.data);
-    p.S = S; p.L = L; p.table_rows = table_rows; p.rot = static_cast<int>(rot);
-    B200_CHECK(Hq + 2 * Hkv < (1 << 24), "%s: too many heads", name);
+    p.L = L; p.table_rows = table_rows; p.S = static_cast<int>(S); p.rot = static_cast<int>(rot);
     p.Hq = static_cast<int>(Hq); p.Hkv = static_cast<int>(Hkv);
-    p.items = B * S * (Hq + 2 * Hkv);
-    const int64_t per_cta = 256 / (D / 8), ctas = (p.items + per_cta - 1) / per_cta;
-    B200_CHECK(ctas < 0x7fffffffLL, "%s: too many elements", name);
+    const bool many = B * S * (Hq + 2 * Hkv) >= kManyRows;
+    const int64_t rows = 256 / (D / (many ? 16 : 8)), passes = (Hq + rows - 1) / rows + (2 * Hkv + rows - 1) / rows;
+    // as many passes as a CTA can have in flight, fewer while there are not two CTAs for every SM
+    int64_t per = kPasses;
+    while (per > 1 && B * S * ((passes + per - 1) / per) < 2 * sm_count()) --per;
+    p.per_cta = static_cast<int>(per);
     cudaStream_t stream = stream_of(ctx);
-    const unsigned grid = static_cast<unsigned>(ctas);
-#define LAUNCH_APPEND(T, DIM)                                                                             \
+    const dim3 grid(static_cast<unsigned>(B * S), static_cast<unsigned>((passes + p.per_cta - 1) / p.per_cta));
+#define LAUNCH_APPEND_H(T, DIM, H)                                                                        \
     do {                                                                                                  \
-        if (interleaved) rope_quant_append_kernel<T, DIM, true><<<grid, 256, 0, stream>>>(p);             \
-        else rope_quant_append_kernel<T, DIM, false><<<grid, 256, 0, stream>>>(p);                        \
+        if (interleaved) rope_quant_append_kernel<T, DIM, true, H><<<grid, 256, 0, stream>>>(p);          \
+        else rope_quant_append_kernel<T, DIM, false, H><<<grid, 256, 0, stream>>>(p);                     \
+    } while (0)
+#define LAUNCH_APPEND(T, DIM)                  \
+    do {                                       \
+        if (many) LAUNCH_APPEND_H(T, DIM, 8);  \
+        else LAUNCH_APPEND_H(T, DIM, 4);       \
     } while (0)
     if (vx.dtype == diopi_dtype_bfloat16) {
         if (D == 128) LAUNCH_APPEND(bf16, 128); else LAUNCH_APPEND(bf16, 64);
@@ -286,6 +411,7 @@ diopiError_t diopiB200RopeQuantAppendKV(diopiContextHandle_t ctx, diopiTensorHan
         if (D == 128) LAUNCH_APPEND(fp16, 128); else LAUNCH_APPEND(fp16, 64);
     }
 #undef LAUNCH_APPEND
+#undef LAUNCH_APPEND_H
     B200_LAUNCH_CHECK(name);
     return diopiSuccess;
 }
@@ -329,13 +455,12 @@ diopiError_t diopiB200DequantKV(diopiContextHandle_t ctx, diopiTensorHandle_t k_
         p.o_sb[i] = outs[i]->stride[0]; p.o_ss[i] = outs[i]->stride[1]; p.o_sh[i] = outs[i]->stride[2];
     }
     p.positions = positions ? static_cast<const int64_t*>(vp.data) : nullptr;
-    p.S = S; p.L = L; p.items = B * S * Hkv;
-    B200_CHECK(Hkv < (1 << 24), "%s: too many heads", name);
-    p.Hkv = static_cast<int>(Hkv);
-    const int64_t per_cta = 256 / (D / 8), ctas = (p.items + per_cta - 1) / per_cta;
-    B200_CHECK(ctas < 0x7fffffffLL, "%s: too many elements", name);
+    B200_CHECK(B * S < 0x7fffffffLL && Hkv < 65536, "%s: too many tokens or heads", name);
+    p.L = L; p.S = static_cast<int>(S); p.Hkv = static_cast<int>(Hkv);
+    p.chunks = static_cast<int>((S + kTokens - 1) / kTokens);
+    const int64_t rows = 256 / (D / 16);
     cudaStream_t stream = stream_of(ctx);
-    const dim3 grid(static_cast<unsigned>(ctas), 2);
+    const dim3 grid(static_cast<unsigned>(B * p.chunks), static_cast<unsigned>((Hkv + rows - 1) / rows));
     if (vko.dtype == diopi_dtype_bfloat16) {
         if (D == 128) dequant_kernel<bf16, 128><<<grid, 256, 0, stream>>>(p); else dequant_kernel<bf16, 64><<<grid, 256, 0, stream>>>(p);
     } else {

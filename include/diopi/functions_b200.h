@@ -103,7 +103,7 @@ DIOPI_API diopiError_t diopiB200RopeAppendKV(diopiContextHandle_t ctx, diopiTens
  *                      scales of the slots positions[b] + s. scale = max|y| / 127, code = y / scale to the nearest (ties to
  *                      even), formed from the fp32 rotation, which is not rounded in between; a row of zeros has scale 0, a
  *                      row that holds an infinity or a NaN gets scale NaN and reads back as NaN. cos / sin: dense float32
- *                      [rows, R / 2] tables indexed by position; the first R (a multiple of 8, at most D) values of a head turn,
+ *                      [rows, R / 2] tables indexed by position; the first R (a multiple of 16, at most D) values of a head turn,
  *                      in pairs (i, i + R / 2) or, `interleaved`, (2i, 2i + 1), the others stay; a long-context scaling of the
  *                      angles is the table's content. Both NULL: nothing is rotated. q_out NULL: qkv holds k and v only.
  *                      A sequence with a negative position is idle: nothing is written for it. Tokens whose slot lies behind

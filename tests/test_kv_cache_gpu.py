@@ -106,7 +106,7 @@ def _check_write(pkg, ctx, B, S, Hq, Hkv, D, rot, L, inter, dtype, positions, se
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("B,S,Hq,Hkv,D,rot,L,inter", [
     (1, 1, 8, 8, 64, 64, 40, False), (3, 1, 4, 2, 128, 128, 33, True), (2, 7, 5, 1, 128, 64, 19, False), (2, 5, 3, 3, 64, 32, 9, True),
-    (4, 2, 2, 1, 128, 8, 6, False), (2, 3, 0, 2, 64, 64, 8, False), (2, 3, 4, 2, 128, 0, 8, False), (1, 200, 6, 2, 128, 32, 256, True)])
+    (4, 2, 2, 1, 128, 16, 6, False), (2, 3, 0, 2, 64, 64, 8, False), (2, 3, 4, 2, 128, 0, 8, False), (1, 200, 6, 2, 128, 32, 256, True)])
 def test_write(pkg, ctx, dtype, B, S, Hq, Hkv, D, rot, L, inter):
     g = torch.Generator().manual_seed(B * 100 + S)
     positions = torch.randint(0, L - S + 1, (B,), generator=g).tolist()
@@ -118,6 +118,15 @@ def test_write(pkg, ctx, dtype, B, S, Hq, Hkv, D, rot, L, inter):
         sl = slice(positions[b], positions[b] + S)
         for out, c, s in ((k, cache.k, cache.ks), (v, cache.v, cache.vs)):   # an fp32 product rounded once: bit for bit
             assert torch.equal(out[b], (c[b, :, sl].float() * s[b, :, sl, None]).to(dtype).transpose(0, 1))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("B,S,Hq,Hkv,D,rot,L,inter", [(2, 300, 40, 9, 128, 128, 310, False), (3, 200, 33, 12, 64, 32, 205, True), (1, 520, 48, 8, 128, 64, 530, True),
+                                                      (2, 400, 0, 21, 64, 16, 402, False)])
+def test_write_many_rows(pkg, ctx, dtype, B, S, Hq, Hkv, D, rot, L, inter):
+    """From 32768 rows on a thread takes 16 values."""
+    assert B * S * (Hq + 2 * Hkv) >= 32768
+    _check_write(pkg, ctx, B, S, Hq, Hkv, D, rot, L, inter, dtype, [3, L - S, -1][:B] if B > 1 else [7], pad=1)
 
 
 def test_write_one_token_two_dimensional(pkg, ctx):
