@@ -180,6 +180,9 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
     constexpr int KS = D / 16;                                    // contraction steps of S^T = tiles of 16 columns of O
     constexpr int NQ = 8 * NT;
     constexpr int ES = QUANT ? 1 : 2;
+    // P in the operand type is as coarse as the result, except for bf16 results over int8 rows, whose P is fp16. There it takes two
+    // terms, P rounded and what the rounding left, in two products: the tensor cores have the time.
+    constexpr int TERMS = QUANT && std::is_same<T, bf16>::value ? 1 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int sh_sum[4], sh_pos[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
         for (int u = 0; u < run; ++u, k0 += kUnit) {
             copies_wait<2 * R::kStages - 1>();
             __syncwarp();
-            uint32_t pb[NT][2];
+            uint32_t pb[TERMS][NT][2];
             const uint8_t* stage = ring + get;
             if (k0 < n) {
                 float s[NT][4], s2[NT][4];
@@ -520,8 +523,18 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                     const float e2 = exp2_approx(s[nt][2] - m[nt][0]), e3 = exp2_approx(s[nt][3] - m[nt][1]);
                     l[nt][0] += e0 + e2;
                     l[nt][1] += e1 + e3;
-                    pb[nt][0] = transpose8x8(Pair<M>::narrow(make_float2(e0 * vs0, e1 * vs0)));
-                    pb[nt][1] = transpose8x8(Pair<M>::narrow(make_float2(e2 * vs1, e3 * vs1)));
+                    float2 lo = make_float2(e0 * vs0, e1 * vs0), hi = make_float2(e2 * vs1, e3 * vs1);   // keys g, g + 8
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        const uint32_t a = Pair<M>::narrow(lo), c = Pair<M>::narrow(hi);
+                        pb[k][nt][0] = transpose8x8(a);
+                        pb[k][nt][1] = transpose8x8(c);
+                        if (k + 1 < TERMS) {
+                            const float2 ra = Pair<M>::widen(a), rc = Pair<M>::widen(c);
+                            lo = make_float2(lo.x - ra.x, lo.y - ra.y);
+                            hi = make_float2(hi.x - rc.x, hi.y - rc.y);
+                        }
+                    }
                 }
             } else {
                 copy_keys();
@@ -558,7 +571,10 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                         a[2] = __byte_perm(vw[2][i], vw[3][i], 0x5410); a[3] = __byte_perm(vw[2][i], vw[3][i], 0x7632);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816<M>(acc[nt][i], a, pb[nt][0], pb[nt][1]);
+                    for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816<M>(acc[nt][i], a, pb[k][nt][0], pb[k][nt][1]);
+                    }
                 }
             }
             get += R::kStage;
