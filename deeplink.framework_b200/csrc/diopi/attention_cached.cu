@@ -34,7 +34,7 @@ namespace {
 constexpr int kUnit = 64;            // keys per unit: 16 for each of a CTA's four warps
 constexpr int kStart = 2;            // what a segment's start and end cost, in units (loading its queries, joining four warps, storing)
 constexpr int kMinPlaces = kStart + 1;   // fewer places than this per CTA are not worth a piece of their own
-constexpr int64_t kWholeKeys = 256;  // caches of at most this capacity: whole segments, one launch
+constexpr int64_t kWholeKeys = 512;  // caches of at most this capacity: whole segments, one launch
 constexpr int64_t kWarpRows = 1024;  // from so many (sequence, query head) pairs on, the join has a warp for each instead of a CTA
 constexpr float kLowest = -3e38f;    // a running maximum before the first score: finite, so that no difference with it is NaN
 constexpr float kGrow = 8.f;         // the running maximum follows only when a score outgrows it by this (log2): P stays below 2^8
@@ -188,7 +188,10 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     grid_launch_dependents();
-    grid_dependency_wait();
+    // Behind a prefix kernel of the same call nothing of that kernel is read here: it lets this one start once ITS wait is over, so
+    // what came before both is complete. This kernel then waits at its end, so that the join, which waits for it, finds both done.
+    const bool late = p.prefix.splits > 0;
+    if (!late) grid_dependency_wait();
 
     // ---- this CTA's range of units ----
     const int W = p.Hkv * p.tiles;
@@ -220,7 +223,10 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
             if (threadIdx.x == 0) p.before[p.B] = all;
         }
         const int total = all * W, ctas = ctas_of(p, total);
-        if (blockIdx.x >= ctas) return;
+        if (blockIdx.x >= ctas) {
+            if (late) grid_dependency_wait();
+            return;
+        }
         const int x0 = place_of(total, blockIdx.x, ctas), x1 = place_of(total, blockIdx.x + 1, ctas);
         // the sequences that hold x0 and x1 (x1 = total: behind the last one)
         if (threadIdx.x == 0) {
@@ -264,7 +270,10 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
             at.left += (over == 0 ? 0 : nb1 - over) - skip;
             if (skip != 0) at.next(p, W);
         }
-        if (at.left <= 0) return;
+        if (at.left <= 0) {
+            if (late) grid_dependency_wait();
+            return;
+        }
     }
 
     // ---- the copies, up to `kStages` tiles ahead of the products, across the ends of segments ----
@@ -680,6 +689,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
         first = false;
     }
     copies_wait<0>();
+    if (late) grid_dependency_wait();
 }
 
 // Joins the pieces of one (sequence, query head): those of the prefix, if there is one, and those of the own keys. WARPS warps take a
