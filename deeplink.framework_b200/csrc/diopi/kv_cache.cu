@@ -17,7 +17,9 @@ namespace b200 {
 namespace {
 
 constexpr int kPasses = 3;         // rows a thread of the writer has in flight
-constexpr int64_t kManyRows = 32768;   // from so many rows on the writer's threads take 16 values instead of 8
+// From so many rows on the writer's threads take 16 values instead of 8: less work around a row (1.57 M rows of 128: 152 us against
+// 179; 98 k: 13.0 against 13.7), but a longer chain (6144 rows: 3.3 us against 3.0; 49 k: 7.9 against 7.8).
+constexpr int64_t kManyRows = 65536;
 constexpr int kTokens = 2;         // tokens a CTA of the read-back takes
 
 struct AppendParams {
@@ -122,8 +124,8 @@ struct Half {
 // partners in the half-split layout, neighbours in the part behind it, for interleaved pairs and for values. The rows of a token come
 // in passes of as many rows as the CTA has groups of D / 2H threads, first those of q, then those of k and v; a CTA takes up to
 // kPasses of them and has their loads in flight together. Whether a pass is q or not is the same for the whole CTA, and a thread's
-// angles serve all its rows. Bound by memory: 2 D bytes in per row, 2 D (q) or D + 4 out. H = 8 halves the work around a row
-// ([16384 tokens, 32 + 2 x 32 heads of 128] 200 -> 155 us), H = 4 is the shorter chain (64 tokens: 5.3 -> 4.3 us).
+// angles serve all its rows. Bound by memory: 2 D bytes in per row, 2 D (q) or D + 4 out; 16384 tokens of 32 + 2 x 32 heads of 128 take
+// 152 us, 4.4 TB/s, with the issue slots two thirds busy. kPasses = 2 needs a second CTA for such a token's three passes: 183 us.
 template <typename T, int D, bool INTERLEAVED, int H>
 __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendParams p) {
     constexpr int LANES = D / (2 * H), ROWS = 256 / LANES;
@@ -241,7 +243,7 @@ struct DequantParams {
 
 // D / 16 threads take a row, 16 values each: a CTA takes 256 / (D / 16) heads of kTokens tokens, of k and of v, with all loads in
 // flight. A code becomes fp32 as the low byte of 2^23 + 128 + code, exactly, and then one product is rounded.
-// Bound by memory: D + 4 bytes in, 2 D out.
+// Bound by memory: D + 4 bytes in, 2 D out; 16384 tokens of 2 x 32 heads of 128 take 80 us, 5.0 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
     constexpr int LANES = D / 16, ROWS = 256 / LANES;

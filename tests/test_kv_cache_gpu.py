@@ -121,11 +121,11 @@ def test_write(pkg, ctx, dtype, B, S, Hq, Hkv, D, rot, L, inter):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
-@pytest.mark.parametrize("B,S,Hq,Hkv,D,rot,L,inter", [(2, 300, 40, 9, 128, 128, 310, False), (3, 200, 33, 12, 64, 32, 205, True), (1, 520, 48, 8, 128, 64, 530, True),
-                                                      (2, 400, 0, 21, 64, 16, 402, False)])
+@pytest.mark.parametrize("B,S,Hq,Hkv,D,rot,L,inter", [(2, 300, 97, 9, 128, 128, 310, False), (3, 200, 65, 23, 64, 32, 205, True), (1, 520, 96, 16, 128, 64, 530, True),
+                                                      (2, 400, 0, 42, 64, 16, 402, False)])
 def test_write_many_rows(pkg, ctx, dtype, B, S, Hq, Hkv, D, rot, L, inter):
-    """From 32768 rows on a thread takes 16 values."""
-    assert B * S * (Hq + 2 * Hkv) >= 32768
+    """From 65536 rows on a thread takes 16 values."""
+    assert B * S * (Hq + 2 * Hkv) >= 65536
     _check_write(pkg, ctx, B, S, Hq, Hkv, D, rot, L, inter, dtype, [3, L - S, -1][:B] if B > 1 else [7], pad=1)
 
 
