@@ -39,9 +39,10 @@ constexpr int kMinPlaces = kStart + 1;   // fewer places than this per CTA are n
 // Caches of at most this capacity: whole segments, one launch (64 x 32 heads of 400 keys: 52 us against 59 with pieces and their join;
 // at 1024 slots one sequence of 8 heads takes 12.9 us whole and 8.6 in pieces).
 constexpr int64_t kWholeKeys = 512;
-// The join has a warp per row up to so many pieces a row (64 sequences x 64 heads, 1 piece: 36 us for the whole call against 54 with a
-// CTA per row), a CTA above (16 x 64 heads, 4 pieces: 38 against 45; 1 x 64 heads, 55 pieces: 40 against 67).
-constexpr int64_t kFewPieces = 3;
+// From so many (sequence, query head) rows on the join has a warp for each, below that a CTA of sixteen (whole calls: 4096 rows of one
+// piece 36 us against 54, 2048 rows of five 93 against 103, 2048 of two 44 either way; 1024 rows of four pieces 44 us against 38, 512
+// of one 99 against 95, 64 of 55 pieces 67 against 40).
+constexpr int64_t kWarpRows = 2048;
 constexpr float kLowest = -3e38f;    // a running maximum before the first score: finite, so that no difference with it is NaN
 constexpr float kGrow = 8.f;         // the running maximum follows only when a score outgrows it by this (log2): P stays below 2^8
 
@@ -804,10 +805,8 @@ cudaError_t launch_attention(const CachedAttnParams& p, int nt, cudaStream_t str
         if (e != cudaSuccess) return e;
     }
     if (p.whole && p.own && p.prefix.splits == 0) return cudaSuccess;
-    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq, segments = static_cast<int64_t>(p.B) * p.Hkv * p.tiles;
-    // pieces of a row: the prefix's, and one per CTA that has units of its segment
-    const int64_t pieces = p.prefix.splits + (p.whole || !p.own ? 1 : p.max_ctas / segments + 1);
-    if (pieces <= kFewPieces) return launch_dependent(cached_attention_join_kernel<T, D, 1>, static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, p, 8 * nt);
+    const int64_t rows = static_cast<int64_t>(p.B) * p.Hq;
+    if (rows >= kWarpRows) return launch_dependent(cached_attention_join_kernel<T, D, 1>, static_cast<unsigned>((rows + 3) / 4), 128, 0, stream, p, 8 * nt);
     return launch_dependent(cached_attention_join_kernel<T, D, 16>, static_cast<unsigned>(rows), 512, 0, stream, p, 8 * nt);
 }
 
