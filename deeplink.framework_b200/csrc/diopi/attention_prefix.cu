@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(384, 1) prefix_attention_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    grid_dependency_wait();     // from here on global memory is read
-    grid_launch_dependents();   // the kernel over the own keys counts on this order
+    grid_launch_dependents();
+    grid_dependency_wait();   // from here on global memory is read
 
     if (warp == 0) {
         if (lane == 0) {

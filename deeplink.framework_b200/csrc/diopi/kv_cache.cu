@@ -305,6 +305,22 @@ bool kv_rows_fit(const TensorView& t, int64_t multiple, bool written) {
     return true;
 }
 
+diopiError_t one_device(const char* name, std::initializer_list<diopiConstTensorHandle_t> tensors) {
+    int current = -1;
+    if (cudaGetDevice(&current) != cudaSuccess) {   // no device at all: the launch will say so
+        (void)cudaGetLastError();
+        current = -1;
+    }
+    for (diopiConstTensorHandle_t t : tensors) {
+        if (t == nullptr) continue;
+        diopiDeviceIndex_t index = 0;
+        B200_CHECK(diopiGetTensorDeviceIndex(t, &index) == diopiSuccess, "%s: host callback failed while reading a tensor's device", name);
+        if (current < 0) current = index;
+        B200_CHECK(index == current, "%s: all tensors must live on one device, the current one (found devices %d and %d)", name, current, static_cast<int>(index));
+    }
+    return diopiSuccess;
+}
+
 diopiError_t kv_cache_check(const char* name, const TensorView& k, const TensorView& ks, const TensorView& v, const TensorView& vs, bool written) {
     B200_CHECK(k.ndim == 4 && v.ndim == 4, "%s: caches must be [batch, kv heads, capacity, dim]", name);
     for (int d = 0; d < 4; ++d) B200_CHECK(k.shape[d] == v.shape[d], "%s: k and v caches must have the same shape", name);
@@ -369,7 +385,9 @@ diopiError_t diopiB200RopeQuantAppendKV(diopiContextHandle_t ctx, diopiTensorHan
         rot = 2 * vc.shape[1];
         B200_CHECK(rot <= D && rot % 16 == 0, "%s: the rotated part (%lld) must be a multiple of 16 and at most the head dim", name, (long long)rot);
     }
+    if (diopiError_t e = one_device(name, {q_out, qkv, cos, sin, positions, k_cache, k_scale, v_cache, v_scale}); e != diopiSuccess) return e;
     if (vx.numel == 0 || L == 0) return diopiSuccess;
+    B200_CHECK(vk.data != vv.data && vks.data != vvs.data, "%s: k and v must have caches and scales of their own", name);
     B200_CHECK(B * S < 0x7fffffffLL && Hq + 2 * Hkv < 65536, "%s: too many tokens or heads", name);
     AppendParams p = {};
     p.qkv = vx.data; p.x_sb = vx.stride[0]; p.x_ss = tokens ? vx.stride[1] : 0;
@@ -445,7 +463,9 @@ diopiError_t diopiB200DequantKV(diopiContextHandle_t ctx, diopiTensorHandle_t k_
     } else {
         B200_CHECK(S <= L, "%s: %lld slots asked of a cache of %lld", name, (long long)S, (long long)L);
     }
+    if (diopiError_t e = one_device(name, {k_out, v_out, k_cache, k_scale, v_cache, v_scale, positions}); e != diopiSuccess) return e;
     if (vko.numel == 0 || L == 0) return diopiSuccess;
+    B200_CHECK(vko.data != vvo.data, "%s: k_out and v_out must be two tensors", name);
     DequantParams p = {};
     const TensorView* caches[2] = {&vk, &vv};
     const TensorView* scales[2] = {&vks, &vvs};

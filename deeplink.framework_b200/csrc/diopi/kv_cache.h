@@ -1,6 +1,8 @@
 // Checks shared by the operators on key / value caches.
 #pragma once
 
+#include <initializer_list>
+
 #include "common.h"
 
 namespace b200 {
@@ -11,5 +13,8 @@ bool kv_rows_fit(const TensorView& t, int64_t multiple, bool written);
 
 // k / v: int8 [batch, kv heads, capacity, dim]; ks / vs: float32 [batch, kv heads, capacity].
 diopiError_t kv_cache_check(const char* name, const TensorView& k, const TensorView& ks, const TensorView& v, const TensorView& vs, bool written);
+
+// All tensors that are given lie on one device, the current one (kernels run there: another device's memory would be a fault).
+diopiError_t one_device(const char* name, std::initializer_list<diopiConstTensorHandle_t> tensors);
 
 }  // namespace b200

@@ -9,6 +9,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <exception>
 
 #include "minihost/minihost_structs.h"
 
@@ -94,7 +95,12 @@ PyObject* call(PyObject* self, PyObject* const* args, Py_ssize_t n) {
                 if (x == Py_None) {
                     a[na++] = 0;
                 } else if (THPVariable_Check(x)) {
-                    if (!describe(f, THPVariable_Unpack(x), &tensors[i])) return nullptr;
+                    try {
+                        if (!describe(f, THPVariable_Unpack(x), &tensors[i])) return nullptr;
+                    } catch (const std::exception& e) {   // a tensor without plain storage or strides
+                        PyErr_SetString(f->error, e.what());
+                        return nullptr;
+                    }
                     a[na++] = reinterpret_cast<uint64_t>(&tensors[i]);
                 } else {   // a handle made by the caller
                     PyObject* p = PyObject_GetAttrString(x, "ptr");

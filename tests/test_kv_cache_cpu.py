@@ -14,7 +14,7 @@ def _handle(diopi, t):
     if not getattr(t, "on_host", False):
         diopi._host.minihostFreeTensor(ctypes.c_void_p(h.ptr))
         shape, stride = ((ctypes.c_int64 * t.dim())(*v) for v in (t.shape, t.stride()))
-        h.ptr = diopi._host.minihostMakeTensor(ctypes.c_void_p(t.data_ptr()), t.dim(), shape, stride, diopi.DTYPE[t.dtype], 1, 0)
+        h.ptr = diopi._host.minihostMakeTensor(ctypes.c_void_p(t.data_ptr()), t.dim(), shape, stride, diopi.DTYPE[t.dtype], 1, getattr(t, "device_index", 0))
     return h
 
 
@@ -60,6 +60,11 @@ def _host(t):
     return t
 
 
+def _elsewhere(t):
+    t.device_index = 1
+    return t
+
+
 def _off(t):
     """The same shape, one element off its alignment."""
     raw = _aligned((t.numel() + 1,), t.dtype)
@@ -98,6 +103,8 @@ _WRITE = [
     ({"sin": _aligned((L + 1, D // 2), F32)}, "float32 tables"),
     ({"k_cache": _aligned((B, HKV, L, 32), I8), "v_cache": _aligned((B, HKV, L, 32), I8)}, "head dim 64 or 128"),
     ({"k_scale": _host(_aligned((B, HKV, L), F32))}, "live on the device"),
+    ({"v_scale": _elsewhere(_aligned((B, HKV, L), F32))}, "one device"),
+    ({"positions": _elsewhere(_aligned((B,), I64))}, "one device"),
 ]
 
 
@@ -113,6 +120,7 @@ def test_write_refuses(diopi, change, match):
     ({"k_out": _aligned((B, L + 1, HKV, D), BF), "v_out": _aligned((B, L + 1, HKV, D), BF), "positions": None}, "slots asked"),
     ({"k_out": _aligned((1, S, HKV, D), BF).expand(B, S, HKV, D)}, "pitches"),
     ({"positions": _aligned((2 * B,), I64)[::2]}, "positions must be"),
+    ({"k_out": _elsewhere(_aligned((B, S, HKV, D), BF))}, "one device"),
 ])
 def test_read_back_refuses(diopi, change, match):
     _refused(diopi, "diopiB200DequantKV", {**_dequant_args(), **change}, match)
@@ -139,6 +147,8 @@ _ATTENTION = [
     ({"softmax_lse": _aligned((B, HQ), BF)}, "softmax_lse"),
     ({"softmax_lse": _aligned((B, 1), F32).expand(B, HQ)}, "softmax_lse"),
     ({"q": _host(_aligned((B, HQ, D), BF))}, "device"),
+    ({"v_cache": _elsewhere(_aligned((B, HKV, L, D), I8))}, "one device"),
+    ({"softmax_lse": _elsewhere(_aligned((B, HQ), F32))}, "one device"),
 ]
 
 
@@ -147,6 +157,14 @@ _ATTENTION = [
 def test_attention_refuses(diopi, entry, change, match):
     args = _attention_args() if entry == "diopiB200CachedAttention" else _prefix_args()
     _refused(diopi, entry, {**args, **change}, match)
+
+
+def test_write_and_read_back_refuse_one_tensor_for_k_and_v(diopi):
+    a = _write_args()
+    _refused(diopi, "diopiB200RopeQuantAppendKV", {**a, "v_cache": a["k_cache"]}, "of their own")
+    _refused(diopi, "diopiB200RopeQuantAppendKV", {**a, "v_scale": a["k_scale"]}, "of their own")
+    d = _dequant_args()
+    _refused(diopi, "diopiB200DequantKV", {**d, "v_out": d["k_out"]}, "two tensors")
 
 
 def test_attention_refuses_out_that_is_q(diopi):
@@ -188,6 +206,9 @@ def test_binding_arguments(diopi):
         diopi.diopiB200CachedAttention(ctx, *list(a.values())[:-1])
     with pytest.raises(diopi.DiopiError, match="no diopi counterpart"):
         diopi.diopiB200CachedAttention(ctx, *{**a, "q": torch.zeros(1, dtype=torch.complex64)}.values())
+    sparse = torch.zeros(2, 2).to_sparse()
+    with pytest.raises(diopi.DiopiError):   # no strides
+        diopi.diopiB200CachedAttention(ctx, *{**a, "q": sparse}.values())
     with pytest.raises(diopi.DiopiError, match="tensor handle is NULL"):
         diopi.diopiB200CachedAttention(ctx, *{**a, "q": None}.values())
     with pytest.raises((TypeError, ValueError)):
