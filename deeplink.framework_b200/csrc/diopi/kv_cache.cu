@@ -120,8 +120,9 @@ struct Half {
     }
 };
 
-// A thread takes 2 H values of a row in two groups: values H c .. H c + H - 1 of the first half of the rotated part and their
-// partners in the half-split layout, neighbours in the part behind it, for interleaved pairs and for values. The rows of a token come
+// A thread takes 2 H values of a row in two groups, one in each half of the part they belong to (the rotated part, the part behind it;
+// a value row is one part): in the half-split layout these are partners, and in every layout the threads of a row touch
+// neighbouring memory with each access. The rows of a token come
 // in passes of as many rows as the CTA has groups of D / 2H threads, first those of q, then those of k and v; a CTA takes up to
 // kPasses of them and has their loads in flight together. Whether a pass is q or not is the same for the whole CTA, and a thread's
 // angles serve all its rows. Bound by memory: 2 D bytes in per row, 2 D (q) or D + 4 out; 16384 tokens of 32 + 2 x 32 heads of 128 take
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendP
     const int64_t start = p.positions[b];
     const int q_passes = (p.Hq + ROWS - 1) / ROWS, first = blockIdx.y * p.per_cta;
     const bool turns = c < p.rot / (2 * H);
-    const int half_lo = !INTERLEAVED && turns ? H * c : 2 * H * c, half_hi = !INTERLEAVED && turns ? p.rot / 2 + H * c : 2 * H * c + H;
+    const int mine_lo = turns ? H * c : p.rot / 2 + H * c, mine_hi = mine_lo + (turns ? p.rot / 2 : (D - p.rot) / 2);
     const T* src = static_cast<const T*>(p.qkv) + b * p.x_sb + s * p.x_ss;
     Half<H> wa[kPasses], wb[kPasses];
 #pragma unroll
@@ -145,23 +146,34 @@ __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendP
         wa[u] = wb[u] = Half<H>{};
         if (u < p.per_cta && h < (pass < q_passes ? p.Hq : p.Hq + 2 * p.Hkv)) {
             const bool is_v = h >= p.Hq + p.Hkv;
-            wa[u].load(src + h * D + (is_v ? 2 * H * c : half_lo));
-            wb[u].load(src + h * D + (is_v ? 2 * H * c + H : half_hi));
+            wa[u].load(src + h * D + (is_v ? H * c : mine_lo));
+            wb[u].load(src + h * D + (is_v ? D / 2 + H * c : mine_hi));
         }
     }
     if (start < 0 || start >= p.L) return;
     const int64_t slot = start + s;
     if (slot >= p.L || (p.rot != 0 && slot >= p.table_rows)) return;
+    // half-split: the angles of the pairs (lo i, hi i); interleaved: those of the lo group's pairs, then of the hi group's
     float2 cs[H / 2], sn[H / 2];
+    if constexpr (INTERLEAVED && H == 4) {
 #pragma unroll
-    for (int i = 0; i < H / 4; ++i) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (turns) {
-            x = *reinterpret_cast<const float4*>(p.cos_t + slot * (p.rot / 2) + H * c + 4 * i);
-            y = *reinterpret_cast<const float4*>(p.sin_t + slot * (p.rot / 2) + H * c + 4 * i);
+        for (int i = 0; i < 2; ++i) {
+            const int64_t at = slot * (p.rot / 2) + 2 * c + i * (p.rot / 4);
+            cs[i] = turns ? *reinterpret_cast<const float2*>(p.cos_t + at) : make_float2(0.f, 0.f);
+            sn[i] = turns ? *reinterpret_cast<const float2*>(p.sin_t + at) : make_float2(0.f, 0.f);
         }
-        cs[2 * i] = make_float2(x.x, x.y); cs[2 * i + 1] = make_float2(x.z, x.w);
-        sn[2 * i] = make_float2(y.x, y.y); sn[2 * i + 1] = make_float2(y.z, y.w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < H / 4; ++i) {
+            const int64_t at = slot * (p.rot / 2) + (INTERLEAVED ? H / 2 * c + i * (p.rot / 4) : H * c + 4 * i);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (turns) {
+                x = *reinterpret_cast<const float4*>(p.cos_t + at);
+                y = *reinterpret_cast<const float4*>(p.sin_t + at);
+            }
+            cs[2 * i] = make_float2(x.x, x.y); cs[2 * i + 1] = make_float2(x.z, x.w);
+            sn[2 * i] = make_float2(y.x, y.y); sn[2 * i + 1] = make_float2(y.z, y.w);
+        }
     }
     T* const q_dst = static_cast<T*>(p.q_out) + b * p.q_sb + s * p.q_ss;
     int8_t* const k_dst = p.cache[0] + b * p.c_sb[0] + slot * p.c_sl[0];
@@ -204,8 +216,8 @@ __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendP
                     hi.w[i] = Pair<T>::narrow(y[H / 2 + i]);
                 }
                 T* dst = q_dst + h * p.q_sh;
-                lo.store(dst + half_lo);
-                hi.store(dst + half_hi);
+                lo.store(dst + mine_lo);
+                hi.store(dst + mine_hi);
             }
         } else {
             float amax = max_abs8(y[0], y[1], y[2], y[3]);
@@ -216,7 +228,7 @@ __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendP
                 const float scale = amax < INFINITY ? amax / 127.f : __uint_as_float(0x7fc00000u);
                 const int hk = is_v ? h - p.Hkv : h;
                 int8_t* dst = (is_v ? v_dst : k_dst) + hk * (is_v ? p.c_sh[1] : p.c_sh[0]);
-                int8_t *lo = dst + (is_v ? 2 * H * c : half_lo), *hi = dst + (is_v ? 2 * H * c + H : half_hi);
+                int8_t *lo = dst + (is_v ? H * c : mine_lo), *hi = dst + (is_v ? D / 2 + H * c : mine_hi);
                 if constexpr (H == 8) {
                     *reinterpret_cast<uint2*>(lo) = quantise({y[0], y[1], y[2], y[3]}, amax, scale);
                     *reinterpret_cast<uint2*>(hi) = quantise({y[4], y[5], y[6], y[7]}, amax, scale);
@@ -241,9 +253,9 @@ struct DequantParams {
     int S, chunks, Hkv;            // chunks of kTokens tokens per sequence
 };
 
-// D / 16 threads take a row, 16 values each: a CTA takes 256 / (D / 16) heads of kTokens tokens, of k and of v, with all loads in
-// flight. A code becomes fp32 as the low byte of 2^23 + 128 + code, exactly, and then one product is rounded.
-// Bound by memory: D + 4 bytes in, 2 D out; 16384 tokens of 2 x 32 heads of 128 take 80 us, 5.0 TB/s.
+// D / 16 threads take a row, 8 values of each half: a CTA takes 256 / (D / 16) heads of kTokens tokens, of k and of v, with all loads
+// in flight. A code becomes fp32 as the low byte of 2^23 + 128 + code, exactly, and then one product is rounded.
+// Bound by memory: D + 4 bytes in, 2 D out; 16384 tokens of 2 x 32 heads of 128 take 65 us, 6.2 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
     constexpr int LANES = D / 16, ROWS = 256 / LANES;
@@ -253,23 +265,24 @@ __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
     if (h >= p.Hkv || start < 0 || start >= p.L || start + s0 >= p.L) return;
     const int64_t slot = start + s0;
     const int tokens = static_cast<int>(min(static_cast<int64_t>(min(kTokens, p.S - s0)), p.L - slot));
-    uint4 v[2][kTokens];
+    uint2 v[2][kTokens][2];
     float f[2][kTokens];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        const int8_t* src = p.cache[w] + b * p.c_sb[w] + h * p.c_sh[w] + slot * p.c_sl[w] + 16 * c;
+        const int8_t* src = p.cache[w] + b * p.c_sb[w] + h * p.c_sh[w] + slot * p.c_sl[w] + 8 * c;
         const float* scales = p.scale[w] + b * p.s_sb[w] + h * p.s_sh[w] + slot;
 #pragma unroll
         for (int t = 0; t < kTokens; ++t) {
             if (t < tokens) {
-                v[w][t] = ld16_stream_raw(src + t * p.c_sl[w]);
+                v[w][t][0] = __ldcs(reinterpret_cast<const uint2*>(src + t * p.c_sl[w]));
+                v[w][t][1] = __ldcs(reinterpret_cast<const uint2*>(src + t * p.c_sl[w] + D / 2));
                 f[w][t] = scales[t];
             }
         }
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        T* out = static_cast<T*>(p.out[w]) + b * p.o_sb[w] + s0 * p.o_ss[w] + h * p.o_sh[w] + 16 * c;
+        T* out = static_cast<T*>(p.out[w]) + b * p.o_sb[w] + s0 * p.o_ss[w] + h * p.o_sh[w] + 8 * c;
 #pragma unroll
         for (int t = 0; t < kTokens; ++t) {
             if (t < tokens) {
@@ -277,7 +290,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
                 const float2 ff = make_float2(f[w][t], f[w][t]), bias = make_float2(-8388736.f, -8388736.f);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t x = word(v[w][t], i) ^ 0x80808080u;
+                    const uint32_t x = ((i & 1) ? v[w][t][i >> 1].y : v[w][t][i >> 1].x) ^ 0x80808080u;
                     const float2 lo = make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7441)));
                     const float2 hi = make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7443)));
                     o[2 * i] = Pair<T>::narrow(mul2(add2(lo, bias), ff));
@@ -285,7 +298,7 @@ __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
                 }
                 T* dst = out + t * p.o_ss[w];
                 *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4*>(dst + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+                *reinterpret_cast<uint4*>(dst + D / 2) = make_uint4(o[4], o[5], o[6], o[7]);
             }
         }
     }
