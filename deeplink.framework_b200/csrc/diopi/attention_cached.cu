@@ -87,10 +87,9 @@ __device__ __forceinline__ int units_of(const CachedAttnParams& p, int b, int* l
     return max(1, (n + kUnit - 1) / kUnit);
 }
 // The dealing works on places: a segment takes kStart places, for what its start and end cost, and then one for each of its units.
-// Of `total` places dealt to `ctas` CTAs, CTA c has [total c / ctas, total (c + 1) / ctas); holder() is the CTA of a place.
+// Of `total` places dealt to `ctas` CTAs, CTA c has [total c / ctas, total (c + 1) / ctas).
 __device__ __forceinline__ int ctas_of(const CachedAttnParams& p, int total) { return min(p.max_ctas, (total + kMinPlaces - 1) / kMinPlaces); }
 __device__ __forceinline__ int place_of(int total, int c, int ctas) { return static_cast<int>(static_cast<int64_t>(total) * c / ctas); }
-__device__ __forceinline__ int holder(int place, int total, int ctas) { return static_cast<int>(((static_cast<int64_t>(place) + 1) * ctas - 1) / total); }
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -714,14 +713,19 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attentio
     if (p.own) {
         const int before = p.before[b], places = p.before[b + 1] - before, total = p.before[p.B] * W;
         const int first = before * W + hw * places, ctas = ctas_of(p, total);
-        c0 = holder(first + kStart, total, ctas);
-        pieces = holder(first + places - 1, total, ctas) - c0 + 1;
+        c0 = place_holder(first + kStart, total, ctas);
+        pieces = place_holder(first + places - 1, total, ctas) - c0 + 1;
         complete = pieces == 1 || p.whole;
         if (complete) pieces = 1;
         if (complete && p.prefix.splits == 0) return;
     }
     const int64_t shared_row = static_cast<int64_t>(hk) * p.prefix.rows + static_cast<int64_t>(b) * p.group + in_group, shared_step = static_cast<int64_t>(p.Hkv) * p.prefix.rows;
-    const int count = p.prefix.splits + pieces;
+    int shared = 0;                  // the prefix's pieces
+    if (p.prefix.splits > 0) {
+        const int at = (hk * p.prefix.row_blocks + static_cast<int>((static_cast<int64_t>(b) * p.group + in_group) / kPrefixRows)) * p.prefix.blocks;
+        shared = place_holder(at + p.prefix.blocks - 1, p.prefix.total, p.prefix.ctas) - place_holder(at, p.prefix.total, p.prefix.ctas) + 1;
+    }
+    const int count = shared + pieces;
     float m = kLowest, l = 0.f, o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = 0.f;
@@ -729,12 +733,12 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attentio
     for (int i = warp; i < count; i += WARPS) {
         const float2* ml;
         const float* src;
-        if (i < p.prefix.splits) {
+        if (i < shared) {
             const int64_t r = i * shared_step + shared_row;
             ml = p.prefix.ml + r;
             src = p.prefix.o + r * D;
         } else {
-            const int j = i - p.prefix.splits;
+            const int j = i - shared;
             const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + static_cast<int64_t>(b) * W + hw : 2 * static_cast<int64_t>(c0 + j) + (j == 0 ? 1 : 0);
             ml = p.part_ml + slot * nq + q;
             src = p.part_o + (slot * nq + q) * D;

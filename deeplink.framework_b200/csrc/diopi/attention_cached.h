@@ -7,15 +7,20 @@
 
 namespace b200 {
 
-// Softmax pieces over the rows of a shared prompt, cut into `splits` ranges of keys: for range s, key head h and query row
-// r = sequence * group + head in group: o[((s * Hkv + h) * rows + r) * D ..], unnormalised, relative to the maximum ml.x (log2);
-// ml.y is the sum of the exponentials.
+// Softmax pieces over the rows of a shared prompt. The blocks of all (key head h, row block) pairs are dealt to `ctas` CTAs in equal
+// ranges; piece i of a pair is what the i-th CTA with blocks of it has. For query row r = sequence * group + head in group:
+// o[((i * Hkv + h) * rows + r) * D ..], unnormalised, relative to the maximum ml.x (log2); ml.y is the sum of the exponentials.
+constexpr int kPrefixRows = 256;       // query rows of a row block
 struct PrefixParts {
     const float* o = nullptr;
     const float2* ml = nullptr;
     int64_t rows = 0;
-    int splits = 0;
+    int splits = 0;                    // pieces a pair has at most; 0: no prefix
+    int blocks = 0, total = 0, ctas = 0, row_blocks = 0;
 };
+
+// The CTA of place `place` among `total` places dealt to `ctas` CTAs; CTA c has [total c / ctas, total (c + 1) / ctas).
+__host__ __device__ __forceinline__ int place_holder(int place, int total, int ctas) { return static_cast<int>(((static_cast<int64_t>(place) + 1) * ctas - 1) / total); }
 
 // A launch that may set itself up while the kernel before it in the stream ends; the kernel waits (grid_dependency_wait) before it
 // touches global memory.

@@ -6,15 +6,18 @@
 // tensor cores: 4 D flops per row and key against 4 D bytes per key, bound by the tensor cores (by the exponentials beside
 // them) from some 200 rows on and by reading the prompt below that.
 //
-// One CTA per (range of keys, key head, 256 query rows), 384 threads, the structure of the prefill kernel (attention.cu):
+// The blocks of 128 keys of all (key head, 256 query rows) pairs, in order, are dealt to at most one CTA per SM in equal consecutive
+// ranges; what a CTA has of one pair is a segment, and every segment leaves its unnormalised fp32 output, running maximum and sum.
+// 384 threads, the structure of the prefill kernel (attention.cu):
 //   warp 0       TMA producer: K and V blocks of 128 keys through a 3-slot ring, the keys one block ahead of the values
 //   warp 1, 3    MMA issuers (one thread each) for row tile 0 and 1: scores and O in TMEM
 //   warp 2       TMEM allocation
 //   warps 4..7   softmax of tile 0, warps 8..11 of tile 1, one thread per row; the two warps of a scheduler take turns at the
 //                exponentials. Before that the same warps copy the tile's query rows into swizzled shared memory: rows of
 //                neighbouring sequences are `group` heads apart in general, which no tensor map describes for every group.
-// The keys are cut into ranges so that the last wave of CTAs is nearly full (plan()); a range leaves its unnormalised fp32 output,
-// running maximum and sum. Every wait is bounded (gemm_sm100.cuh); a time-out ends the kernel and raises the status word.
+// The ring and the barriers run on from one segment to the next. Every wait is bounded (gemm_sm100.cuh); a time-out ends the kernel
+// and raises the status word. 256 sequences x 64 heads behind 32768 tokens,
+// 8 key heads of 128: 288 us, 955 TFLOP/s at 1.59 GHz. Shared memory is the tightest: both products read both operands there.
 #include <cuda.h>
 
 #include <cmath>
@@ -49,7 +52,8 @@ struct PrefixParams {
     const void* q;
     int64_t q_sb, q_sh;
     int rows, group, Hkv, P;
-    int row_blocks, blocks_per_split;
+    int row_blocks, blocks;            // blocks of keys
+    int total, ctas;                   // blocks of all pairs, CTAs they are dealt to
     int k_hfirst, v_hfirst;            // order of the tensor maps' head and row dimensions
     float scale_log2;
     uint32_t idesc_s, idesc_pv;
@@ -88,19 +92,28 @@ __global__ void __launch_bounds__(384, 1) prefix_attention_kernel(const __grid_c
     volatile uint32_t* abort_flag = tmem_slot + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // the row blocks that share a range of keys are neighbours, so that its K / V blocks stay in L2
-    const int rb = blockIdx.x % p.row_blocks;
-    const int rest = blockIdx.x / p.row_blocks;
-    const int hk = rest % p.Hkv, split = rest / p.Hkv;
-    const int q0 = rb * 2 * kTile;
-    const int blk0 = split * p.blocks_per_split;
-    const int n = min(p.blocks_per_split, (p.P + kBlock - 1) / kBlock - blk0);   // >= 1 by the launch
-    const int n1 = q0 + kTile < p.rows ? n : 0;                                  // tile 1 may have no rows
+    const int x0 = static_cast<int>(static_cast<int64_t>(p.total) * blockIdx.x / p.ctas), x1 = static_cast<int>(static_cast<int64_t>(p.total) * (blockIdx.x + 1) / p.ctas);
+    // The CTA's segment that starts at place x: key head, first query row, first block, blocks; n1: those of tile 1, which has no rows in
+    // the last row block of some batches.
+    struct Segment {
+        int hk, q0, blk0, n, n1, piece;
+    };
+    auto segment = [&](int x) {
+        Segment g;
+        const int pair = x / p.blocks;
+        g.hk = pair / p.row_blocks;
+        g.q0 = (pair - g.hk * p.row_blocks) * 2 * kTile;
+        g.blk0 = x - pair * p.blocks;
+        g.n = min(p.blocks - g.blk0, x1 - x);
+        g.n1 = g.q0 + kTile < p.rows ? g.n : 0;
+        g.piece = static_cast<int>(blockIdx.x) - place_holder(pair * p.blocks, p.total, p.ctas);
+        return g;
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kRing; ++s) {
             mbar_init(&kv_full[s], 1);
-            mbar_init(&kv_empty[s], 2);   // one arrival per tile (a tile that is alone arrives twice)
+            mbar_init(&kv_empty[s], 2);   // one arrival per tile
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 4);
@@ -129,205 +142,233 @@ __global__ void __launch_bounds__(384, 1) prefix_attention_kernel(const __grid_c
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int r = 0; r < 2 * n; ++r) {
-                const int slot = r % kRing;
-                if (!mbar_wait(&kv_empty[slot], (static_cast<uint32_t>(r / kRing) & 1u) ^ 1u, abort_flag)) break;
-                mbar_arrive_expect_tx(&kv_full[slot], S::kTileBytes);
-                const bool is_v = r == 2 * n - 1 || (r != 0 && (r & 1) == 0);
-                const int blk = is_v ? (r == 2 * n - 1 ? n - 1 : (r - 2) / 2) : (r + 1) / 2;
-                const int row = (blk0 + blk) * kBlock;   // rows behind the prompt are filled with zeros by the copy engine
-                const int hfirst = is_v ? p.v_hfirst : p.k_hfirst;
-                for (int c = 0; c < D / 64; ++c) {
-                    tma_load_4d(smem_kv + slot * S::kTileBytes + c * kHalf, is_v ? &map_v : &map_k, &kv_full[slot], c * 64, hfirst ? hk : row, hfirst ? row : hk, 0);
+            bool ok = true;
+            int base = 0;   // loads of the segments before
+            for (int x = x0; x < x1 && ok;) {
+                const Segment g = segment(x);
+                for (int r = 0; r < 2 * g.n; ++r) {
+                    const int slot = (base + r) % kRing;
+                    ok = mbar_wait(&kv_empty[slot], (static_cast<uint32_t>((base + r) / kRing) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&kv_full[slot], S::kTileBytes);
+                    const bool is_v = r == 2 * g.n - 1 || (r != 0 && (r & 1) == 0);
+                    const int blk = is_v ? (r == 2 * g.n - 1 ? g.n - 1 : (r - 2) / 2) : (r + 1) / 2;
+                    const int row = (g.blk0 + blk) * kBlock;   // rows behind the prompt are filled with zeros by the copy engine
+                    const int hfirst = is_v ? p.v_hfirst : p.k_hfirst;
+                    for (int c = 0; c < D / 64; ++c) {
+                        tma_load_4d(smem_kv + slot * S::kTileBytes + c * kHalf, is_v ? &map_v : &map_k, &kv_full[slot], c * 64, hfirst ? g.hk : row, hfirst ? row : g.hk, 0);
+                    }
                 }
+                base += 2 * g.n;
+                x += g.n;
             }
         }
     } else if (warp == 1 || warp == 3) {
         if (lane == 0) {
             const int t = warp == 1 ? 0 : 1;
-            const int n_t = t == 0 ? n : n1, n_o = t == 0 ? n1 : n;
-            bool ok = n_t > 0 && mbar_wait(&q_full[t], 0, abort_flag);
-            auto release = [&](int slot, int j) {
-                umma_commit(&kv_empty[slot]);
-                if (n_o <= j) umma_commit(&kv_empty[slot]);
-            };
-            auto scores = [&](int j) -> bool {
-                const int r = load_of_k(j), slot = r % kRing;
-                if (j > 0 && !mbar_wait(&s_free[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag)) return false;
-                if (!mbar_wait(&kv_full[slot], static_cast<uint32_t>(r / kRing) & 1u, abort_flag)) return false;
-                tc_fence_after();
-                const uint32_t qa = smem_u32(smem_q + t * S::kTileBytes), ka = smem_u32(smem_kv + slot * S::kTileBytes);
+            bool ok = true;
+            int base = 0, done = 0, queries = 0;   // loads, blocks of this tile and tiles of queries of the segments before
+            for (int x = x0; x < x1 && ok;) {
+                const Segment g = segment(x);
+                const int n_t = t == 0 ? g.n : g.n1;
+                auto scores = [&](int j) -> bool {
+                    const int r = base + load_of_k(j), slot = r % kRing;
+                    if (done + j > 0 && !mbar_wait(&s_free[t], static_cast<uint32_t>(done + j - 1) & 1u, abort_flag)) return false;
+                    if (!mbar_wait(&kv_full[slot], static_cast<uint32_t>(r / kRing) & 1u, abort_flag)) return false;
+                    tc_fence_after();
+                    const uint32_t qa = smem_u32(smem_q + t * S::kTileBytes), ka = smem_u32(smem_kv + slot * S::kTileBytes);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-                    umma_f16_ss(tmem_base + t * 128, make_smem_desc_sw128(qa + off, 16, 1024), make_smem_desc_sw128(ka + off, 16, 1024), p.idesc_s, k != 0 ? 1u : 0u);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
+                        umma_f16_ss(tmem_base + t * 128, make_smem_desc_sw128(qa + off, 16, 1024), make_smem_desc_sw128(ka + off, 16, 1024), p.idesc_s, k != 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[t]);
+                    umma_commit(&kv_empty[slot]);
+                    return true;
+                };
+                // A tile without rows hands the blocks straight back: it has to see every phase of the ring's barriers, since a wait names a
+                // phase by its parity only and would take one two phases back for the one it means.
+                for (int r = base; n_t == 0 && ok && r < base + 2 * g.n; ++r) {
+                    ok = mbar_wait(&kv_full[r % kRing], static_cast<uint32_t>(r / kRing) & 1u, abort_flag);
+                    if (ok) mbar_arrive(&kv_empty[r % kRing]);
                 }
-                umma_commit(&s_full[t]);
-                release(slot, j);
-                return true;
-            };
-            if (ok) ok = scores(0);
-            for (int j = 0; j < n_t && ok; ++j) {
-                if (j + 1 < n_t && !scores(j + 1)) break;
-                const int r = load_of_v(j, n), slot = r % kRing;
-                if (!mbar_wait(&p_full[t], static_cast<uint32_t>(j) & 1u, abort_flag)) break;
-                if (!mbar_wait(&kv_full[slot], static_cast<uint32_t>(r / kRing) & 1u, abort_flag)) break;
-                tc_fence_after();
-                const uint32_t pa = smem_u32(smem_p + t * kPBytes), va = smem_u32(smem_kv + slot * S::kTileBytes);
+                if (n_t > 0) ok = mbar_wait(&q_full[t], static_cast<uint32_t>(queries) & 1u, abort_flag) && scores(0);
+                for (int j = 0; j < n_t && ok; ++j) {
+                    if (j + 1 < n_t && !(ok = scores(j + 1))) break;
+                    const int r = base + load_of_v(j, g.n), slot = r % kRing;
+                    ok = mbar_wait(&p_full[t], static_cast<uint32_t>(done + j) & 1u, abort_flag) &&
+                         mbar_wait(&kv_full[slot], static_cast<uint32_t>(r / kRing) & 1u, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t pa = smem_u32(smem_p + t * kPBytes), va = smem_u32(smem_kv + slot * S::kTileBytes);
 #pragma unroll
-                for (int k = 0; k < kBlock / 16; ++k) {
-                    // V is N-contiguous: 16 keys are 16 rows of 128 bytes; with two column halves they lie kHalf apart
-                    umma_f16_ss(tmem_base + 256 + t * 128, make_smem_desc_sw128(pa + (k >> 2) * kHalf + (k & 3) * 32, 16, 1024),
-                                make_smem_desc_sw128(va + k * 2048, kHalf, 1024), p.idesc_pv, (j > 0 || k != 0) ? 1u : 0u);
+                    for (int k = 0; k < kBlock / 16; ++k) {
+                        // V is N-contiguous: 16 keys are 16 rows of 128 bytes; with two column halves they lie kHalf apart
+                        umma_f16_ss(tmem_base + 256 + t * 128, make_smem_desc_sw128(pa + (k >> 2) * kHalf + (k & 3) * 32, 16, 1024),
+                                    make_smem_desc_sw128(va + k * 2048, kHalf, 1024), p.idesc_pv, (j > 0 || k != 0) ? 1u : 0u);
+                    }
+                    umma_commit(&pv_done[t]);
+                    umma_commit(&kv_empty[slot]);
                 }
-                umma_commit(&pv_done[t]);
-                release(slot, j);
+                base += 2 * g.n;
+                done += n_t;
+                queries += n_t > 0 ? 1 : 0;
+                x += g.n;
             }
         }
     } else if (warp >= 4) {
         const int t = (warp - 4) >> 2, quarter = warp & 3, r_in_tile = quarter * 32 + lane;
-        const int n_t = t == 0 ? n : n1;
-        const int row = q0 + t * kTile + r_in_tile;
-        if (n_t > 0) {
-            // the tile's query rows, 16 bytes a thread; chunk c of a row sits at c ^ (row & 7) of its 128-byte line
-            for (int i = r_in_tile; i < kTile * (D / 8); i += 128) {
-                const int r = i / (D / 8), c = i - r * (D / 8), qr = q0 + t * kTile + r;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (qr < p.rows) {
-                    const int b = qr / p.group, g = qr - b * p.group;
-                    w = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(hk * p.group + g) * p.q_sh + c * 8);
-                }
-                *reinterpret_cast<uint4*>(smem_q + t * S::kTileBytes + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) * 16)) = w;
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[t]);
-        }
         uint8_t* pbuf = smem_p + t * kPBytes;
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t s_tmem = lane_base + t * 128, o_tmem = lane_base + 256 + t * 128;
-        float m_used = -INFINITY, l_sum = 0.f;
         bool ok = true;
-        for (int j = 0; j < n_t; ++j) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], static_cast<uint32_t>(j) & 1u, abort_flag))) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + c * 32, s[c]);
-            tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[t]);
-            const int left = p.P - (blk0 + j) * kBlock;   // keys of this block
-            if (left < kBlock) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (c * 32 + i >= left) s[c][i] = __float_as_uint(-INFINITY);
+        int done = 0, turns = 0;   // blocks of this tile, and blocks that both tiles have, of the segments before
+        for (int x = x0; x < x1 && ok;) {
+            const Segment g = segment(x);
+            const int n_t = t == 0 ? g.n : g.n1;
+            const bool both = g.n1 > 0;
+            const int row = g.q0 + t * kTile + r_in_tile;
+            if (n_t > 0) {
+                // The tile's query rows, 16 bytes a thread; chunk c of a row sits at c ^ (row & 7) of its 128-byte line. The products over the
+                // previous segment's queries are over: this warp has seen their last scores.
+                for (int i = r_in_tile; i < kTile * (D / 8); i += 128) {
+                    const int r = i / (D / 8), c = i - r * (D / 8), qr = g.q0 + t * kTile + r;
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (qr < p.rows) {
+                        const int b = qr / p.group, h = qr - b * p.group;
+                        w = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(g.hk * p.group + h) * p.q_sh + c * 8);
                     }
+                    *reinterpret_cast<uint4*>(smem_q + t * S::kTileBytes + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) * 16)) = w;
                 }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[t]);
             }
-            float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[c][i]));
-            }
-            const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scale_log2;
-            bool rescale = false;
-            float factor = 1.f;
-            if (j == 0) {
-                m_used = mx;
-            } else {
-                rescale = __any_sync(0xffffffffu, mx > m_used + kRescale);
-                if (rescale) {
-                    const float m_new = fmaxf(m_used, mx);
-                    factor = (m_used == -INFINITY) ? 0.f : exp2_approx(m_used - m_new);
-                    m_used = m_new;
-                    l_sum *= factor;
-                }
-            }
-            const float base = (m_used == -INFINITY) ? 0.f : m_used;
-            // tile 0 block j, tile 1 block j, tile 0 block j + 1, ...: turns at the exponentials, as far as both tiles exist
-            bool go = true;
-            if (t == 0) {
-                if (j > 0 && n1 > 0) go = mbar_wait(&turn[quarter * 2], static_cast<uint32_t>(j - 1) & 1u, abort_flag);
-            } else {
-                go = mbar_wait(&turn[quarter * 2 + 1], static_cast<uint32_t>(j) & 1u, abort_flag);
-            }
-            if (!__all_sync(0xffffffffu, go)) {
-                ok = false;
-                break;
-            }
-            float parts[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    float e[8];
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        e[u] = exp2_approx(fmaf(__uint_as_float(s[c][i + u]), p.scale_log2, -base));
-                        parts[u & 3] += e[u];
-                    }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) s[c][i / 2 + u] = Pair<T>::narrow(make_float2(e[2 * u], e[2 * u + 1]));
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&turn[quarter * 2 + (t == 0 ? 1 : 0)]);
-            if (j > 0) {   // P of the previous block has been consumed and O is at rest
-                if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], static_cast<uint32_t>(j - 1) & 1u, abort_flag))) {
+            float m_used = -INFINITY, l_sum = 0.f;
+            for (int j = 0; j < n_t; ++j) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], static_cast<uint32_t>(done + j) & 1u, abort_flag))) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + c * 32, s[c]);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[t]);
+                const int left = p.P - (g.blk0 + j) * kBlock;   // keys of this block
+                if (left < kBlock) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (c * 32 + i >= left) s[c][i] = __float_as_uint(-INFINITY);
+                        }
+                    }
+                }
+                float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[c][i]));
+                }
+                const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * p.scale_log2;
+                bool rescale = false;
+                float factor = 1.f;
+                if (j == 0) {
+                    m_used = mx;
+                } else {
+                    rescale = __any_sync(0xffffffffu, mx > m_used + kRescale);
+                    if (rescale) {
+                        const float m_new = fmaxf(m_used, mx);
+                        factor = (m_used == -INFINITY) ? 0.f : exp2_approx(m_used - m_new);
+                        m_used = m_new;
+                        l_sum *= factor;
+                    }
+                }
+                const float base = (m_used == -INFINITY) ? 0.f : m_used;
+                // tile 0 block j, tile 1 block j, tile 0 block j + 1, ...: turns at the exponentials, as far as both tiles exist
+                bool go = true;
+                if (both && t == 0 && turns + j > 0) go = mbar_wait(&turn[quarter * 2], static_cast<uint32_t>(turns + j - 1) & 1u, abort_flag);
+                if (both && t == 1) go = mbar_wait(&turn[quarter * 2 + 1], static_cast<uint32_t>(turns + j) & 1u, abort_flag);
+                if (!__all_sync(0xffffffffu, go)) {
+                    ok = false;
+                    break;
+                }
+                float parts[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float e[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            e[u] = exp2_approx(fmaf(__uint_as_float(s[c][i + u]), p.scale_log2, -base));
+                            parts[u & 3] += e[u];
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) s[c][i / 2 + u] = Pair<T>::narrow(make_float2(e[2 * u], e[2 * u + 1]));
+                    }
+                }
+                __syncwarp();
+                if (both && lane == 0) mbar_arrive(&turn[quarter * 2 + (t == 0 ? 1 : 0)]);
+                if (j > 0) {   // P of the previous block has been consumed and O is at rest
+                    if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[t], static_cast<uint32_t>(done + j - 1) & 1u, abort_flag))) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                }
+                if (rescale) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(o_tmem + c * 32, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                        tmem_st_32x32(o_tmem + c * 32, o);
+                    }
+                    tmem_st_wait();
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        const int col = c * 32 + i, chunk = (col & 63) >> 3;
+                        *reinterpret_cast<uint4*>(pbuf + (col >> 6) * kHalf + r_in_tile * 128 + ((chunk ^ (r_in_tile & 7)) * 16)) =
+                            make_uint4(s[c][i / 2], s[c][i / 2 + 1], s[c][i / 2 + 2], s[c][i / 2 + 3]);
+                    }
+                }
+                l_sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
+                fence_proxy_async();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
             }
-            if (rescale) {
+            if (ok && n_t > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], static_cast<uint32_t>(done + n_t - 1) & 1u, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                const int64_t at = (static_cast<int64_t>(g.piece) * p.Hkv + g.hk) * p.rows + row;
+                if (row < p.rows) p.ml[at] = make_float2(m_used, l_sum);
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
                     tmem_ld_32x32(o_tmem + c * 32, o);
                     tmem_ld_wait();
+                    if (row < p.rows) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                    tmem_st_32x32(o_tmem + c * 32, o);
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(p.o + at * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
                 }
-                tmem_st_wait();
+                tc_fence_before();   // O is read before the next segment's first product overwrites it
             }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    const int col = c * 32 + i, chunk = (col & 63) >> 3;
-                    *reinterpret_cast<uint4*>(pbuf + (col >> 6) * kHalf + r_in_tile * 128 + ((chunk ^ (r_in_tile & 7)) * 16)) =
-                        make_uint4(s[c][i / 2], s[c][i / 2 + 1], s[c][i / 2 + 2], s[c][i / 2 + 3]);
-                }
-            }
-            l_sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
-            fence_proxy_async();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
-        }
-        if (ok && n_t > 0 && __all_sync(0xffffffffu, mbar_wait(&pv_done[t], static_cast<uint32_t>(n_t - 1) & 1u, abort_flag))) {
-            tc_fence_after();
-            const int64_t at = (static_cast<int64_t>(split) * p.Hkv + hk) * p.rows + row;
-            if (row < p.rows) p.ml[at] = make_float2(m_used, l_sum);
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld_32x32(o_tmem + c * 32, o);
-                tmem_ld_wait();
-                if (row < p.rows) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(p.o + at * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                }
-            }
+            done += n_t;
+            turns += both ? g.n : 0;
+            x += g.n;
         }
     }
 
@@ -362,22 +403,25 @@ bool map_of(const TensorView& t, CUtensorMap* map, int* hfirst) {
     return tc_encode_map4(reinterpret_cast<::CUtensorMap_st*>(map), t.dtype, t.data, dims, pitches, hf ? 1 : kBlock, hf ? kBlock : 1);
 }
 
-// Ranges of keys. More ranges fill the last wave of CTAs better; each costs a CTA's set-up and its fp32 pieces, which are written and
-// read back. In microseconds: 2 for a block of a CTA (two 128 x 128 x D products for each of two tiles, or 64 KiB at a 148th of
-// the memory rate), 4 for a CTA's start and end, 5 TB/s for the pieces.
-int plan(int64_t ctas, int64_t blocks, int64_t piece_bytes, int sms) {
-    double best = 0.0;
-    int best_per = static_cast<int>(blocks);
-    for (int64_t s = 1; s <= blocks && s <= 2 * sms; ++s) {
-        const int64_t per = (blocks + s - 1) / s, splits = (blocks + per - 1) / per;
-        const double waves = static_cast<double>((ctas * splits + sms - 1) / sms);
-        const double cost = waves * (2.0 * per + 4.0) + static_cast<double>(splits) * piece_bytes * 2 / 5e6;
-        if (s == 1 || cost < best) {
-            best = cost;
-            best_per = static_cast<int>(per);
-        }
+// CTAs the blocks are dealt to: a multiple of the pairs (each pair in as many equal ranges), or all SMs (ranges that cross from one pair
+// to the next) where no multiple comes near. All SMs pay only for a large gap, because the power limit lowers the clock with
+// every SM that multiplies: 300 sequences x 64 heads (80 pairs) behind 8192 tokens take 135 us on 148 SMs and 168 on 80, 256 behind
+// 32768 (64 pairs) 340 us on 148 as on 128, 128 behind 16384 (32 pairs) 111 and 100. In microseconds: 2 for a block of a CTA (two 128 x 128 x D products for each of two tiles, or 64 KiB at a 148th of the
+// memory rate), 4 for a segment's start and end, 5 TB/s for the fp32 pieces, written and read back.
+int plan(int64_t pairs, int64_t blocks, int64_t piece_bytes, int sms) {
+    const int64_t total = pairs * blocks;
+    auto cost = [&](int64_t ctas) {
+        const double pieces = static_cast<double>(ctas) / pairs + (ctas % pairs == 0 ? 0.0 : 1.0);
+        const double segments = ctas % pairs == 0 ? 1.0 : static_cast<double>(pairs) / ctas + 1.0;
+        return 2.0 * ((total + ctas - 1) / ctas) + 4.0 * segments + pieces * piece_bytes * 2 / 5e6;
+    };
+    const int64_t all = total < sms ? total : sms;
+    int64_t best = 0;
+    for (int64_t ctas = pairs; ctas <= all; ctas += pairs) {
+        if (best == 0 || cost(ctas) < cost(best)) best = ctas;
     }
-    return best_per;
+    if (best == 0 || 1.25 * cost(all) < cost(best)) best = all;
+    return static_cast<int>(best);
 }
 
 }  // namespace
@@ -390,10 +434,12 @@ diopiError_t prefix_attention(const char* name, diopiContextHandle_t ctx, const 
     p.rows = static_cast<int>(rows); p.group = static_cast<int>(group); p.Hkv = static_cast<int>(Hkv); p.P = static_cast<int>(P);
     p.row_blocks = static_cast<int>((rows + 2 * kTile - 1) / (2 * kTile));
     p.scale_log2 = scale_log2;
-    const int64_t blocks = (P + kBlock - 1) / kBlock, ctas = Hkv * p.row_blocks;
-    p.blocks_per_split = plan(ctas, blocks, rows * Hkv * (D * 4 + 8), sm_count());
-    const int64_t splits = (blocks + p.blocks_per_split - 1) / p.blocks_per_split;
-    B200_CHECK(ctas * splits < 0x7fffffffLL, "%s: too many query rows", name);
+    const int64_t blocks = (P + kBlock - 1) / kBlock, pairs = Hkv * p.row_blocks;
+    B200_CHECK(pairs * blocks < 0x7fffffffLL, "%s: too many query rows", name);
+    p.blocks = static_cast<int>(blocks);
+    p.total = static_cast<int>(pairs * blocks);
+    p.ctas = plan(pairs, blocks, rows * Hkv * (D * 4 + 8), sm_count());
+    const int64_t splits = (blocks - 1) * p.ctas / p.total + 2;   // pieces a pair has at most
     const int fmt = q.dtype == diopi_dtype_bfloat16 ? 1 : 0;
     p.idesc_s = make_idesc_f16(fmt, false, kTile, kBlock);
     p.idesc_pv = make_idesc_f16(fmt, true, kTile, static_cast<int>(D));
@@ -407,7 +453,7 @@ diopiError_t prefix_attention(const char* name, diopiContextHandle_t ctx, const 
     B200_CHECK(diopiGetTensorData(ws, &ptr) == diopiSuccess && ptr != nullptr, "%s: workspace has no data pointer", name);
     p.o = static_cast<float*>(ptr);
     p.ml = reinterpret_cast<float2*>(p.o + splits * Hkv * rows * D);
-    const unsigned grid = static_cast<unsigned>(ctas * splits);
+    const unsigned grid = static_cast<unsigned>(p.ctas);
     cudaError_t e;
     if (fmt == 1) e = D == 128 ? launch<bf16, 128>(mk, mv, p, grid, stream) : launch<bf16, 64>(mk, mv, p, grid, stream);
     else e = D == 128 ? launch<fp16, 128>(mk, mv, p, grid, stream) : launch<fp16, 64>(mk, mv, p, grid, stream);
@@ -415,7 +461,8 @@ diopiError_t prefix_attention(const char* name, diopiContextHandle_t ctx, const 
         (void)cudaGetLastError();
         B200_FAIL("%s: kernel launch failed: %s", name, cudaGetErrorString(e));
     }
-    parts->o = p.o; parts->ml = p.ml; parts->rows = rows; parts->splits = static_cast<int>(splits);
+    parts->o = p.o; parts->ml = p.ml; parts->rows = rows;
+    parts->splits = static_cast<int>(splits); parts->blocks = p.blocks; parts->total = p.total; parts->ctas = p.ctas; parts->row_blocks = p.row_blocks;
     return diopiSuccess;
 }
 

@@ -361,6 +361,15 @@ def test_shared_prefix(pkg, ctx, dtype, P, Hq, Hkv, D):
     _attend(pkg, ctx, dtype, 5, Hq, Hkv, D, 70, [70, 0, 1, 33, 64], quant=(P != 127), P=P, heads_first=P == 300)
 
 
+@pytest.mark.parametrize("quant", [True, False])
+def test_shared_prefix_ranges_across_pairs(pkg, ctx, quant):
+    """More (key head, 256 query rows) pairs than half the SMs, and than all of them: a CTA's range of blocks crosses from one pair into
+    the next, and from pairs with two row tiles into the last one of a head, which has one."""
+    _attend(pkg, ctx, BF, 550, 32, 16, 64, 8, [i % 9 for i in range(550)], quant, P=2560)
+    _attend(pkg, ctx, FP, 275, 128, 32, 64, 8, [i % 9 for i in range(275)], quant, P=200)
+    _attend(pkg, ctx, BF, 265, 80, 80, 128, 8, [i % 9 for i in range(265)], quant, P=300)
+
+
 @pytest.mark.parametrize("B,Hq,Hkv,D,P", [(70, 8, 4, 128, 500), (300, 2, 2, 64, 130), (33, 16, 1, 128, 1025), (129, 2, 1, 128, 64), (2, 2, 2, 128, 9000)])
 @pytest.mark.parametrize("quant", [True, False])
 def test_shared_prefix_many_rows(pkg, ctx, quant, B, Hq, Hkv, D, P):
