@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
         const int per = (p.B + 127) / 128;
         const int b_lo = min(p.B, static_cast<int>(threadIdx.x) * per), b_hi = min(p.B, b_lo + per);
         int mine = 0, n = 0;
+#pragma unroll 4
         for (int i = b_lo; i < b_hi; ++i) mine += kStart + units_of(p, i, &n);
         int incl = mine;
 #pragma unroll
@@ -222,6 +223,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
         }
         if (blockIdx.x == 0 && p.before != nullptr) {
             int x = excl;
+#pragma unroll 4
             for (int i = b_lo; i < b_hi; ++i) {
                 p.before[i] = x;
                 x += kStart + units_of(p, i, &n);

@@ -272,7 +272,7 @@ def test_cached_attention(pkg, ctx, quant, dtype, Hq, Hkv, D):
 
 
 @pytest.mark.parametrize("quant", [True, False])
-@pytest.mark.parametrize("B,Hq,Hkv,L,lo", [(1, 8, 1, 9001, 9001), (2, 2, 2, 5000, 1), (3, 40, 8, 2049, 2000), (1, 1, 1, 20000, 19999), (40, 8, 4, 700, 1)])
+@pytest.mark.parametrize("B,Hq,Hkv,L,lo", [(1, 8, 1, 9001, 9001), (2, 2, 2, 5000, 1), (3, 40, 8, 2049, 2000), (1, 1, 1, 20000, 19999), (40, 8, 4, 700, 1), (700, 2, 1, 530, 0)])
 def test_cached_attention_long_and_uneven(pkg, ctx, quant, B, Hq, Hkv, L, lo):
     g = torch.Generator().manual_seed(L)
     _attend(pkg, ctx, BF, B, Hq, Hkv, 128, L, torch.randint(lo, L + 1, (B,), generator=g).tolist(), quant)
