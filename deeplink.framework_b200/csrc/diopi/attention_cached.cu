@@ -14,7 +14,7 @@
 // segment) and a second kernel joins them in a fixed order - no atomics, the same bits every time.
 //
 // A warp takes 16 keys of a unit. Asynchronous copies bring its rows into a ring of its own in shared memory, two or three tiles ahead
-// and across the ends of segments: 100 KB in flight on an SM, where register loads held 30 (427 -> 352 us). The products run on
+// and across the ends of segments: some 100 KB in flight on an SM, where register loads held a third (427 -> 354 us). The products run on
 // mma.sync.m16n8k16 with the KEYS as the 16 rows and the query heads as the 8 columns: S^T = K Q^T, O^T = V^T P^T. At a few flops per
 // byte a larger instruction would not be filled; what this shape saves is the feeding, because the order of the contracted index is
 // free. For S^T a lane takes 16-byte chunks of its two key rows and the queries are laid out the same way; for O^T a lane takes 16
@@ -36,7 +36,8 @@ namespace {
 
 constexpr int kUnit = 64;            // keys per unit: 16 for each of a CTA's four warps
 // What a segment's start and end cost, in units (loading its queries, joining four warps, storing). Ragged batch of 44 sequences, 1 to
-// 16384 keys, int8: 164 / 166 / 137 / 133 / 137 us with 0 / 1 / 2 / 3 / 5; 64 own caches of 1 to 1024 keys: 137 / 108 / 94 / 96 / 100.
+// 16384 keys, int8: 164 / 166 / 137 / 133 / 137 us with 0 / 1 / 2 / 3 / 5; 64 sequences of 1 to 1024 own keys
+// behind a prompt: 137 / 108 / 94 / 96 / 100.
 constexpr int kStart = 2;
 constexpr int kMinPlaces = kStart + 1;   // fewer places than this per CTA are not worth a piece of their own
 // Caches of at most this capacity: whole segments, one launch (64 x 32 heads of 400 keys: 52 us against 59 with pieces and their join;

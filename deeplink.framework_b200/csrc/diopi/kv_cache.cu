@@ -126,7 +126,7 @@ struct Half {
 // in passes of as many rows as the CTA has groups of D / 2H threads, first those of q, then those of k and v; a CTA takes up to
 // kPasses of them and has their loads in flight together. Whether a pass is q or not is the same for the whole CTA, and a thread's
 // angles serve all its rows. Bound by memory: 2 D bytes in per row, 2 D (q) or D + 4 out; 16384 tokens of 32 + 2 x 32 heads of 128 take
-// 152 us, 4.4 TB/s, with the issue slots two thirds busy. kPasses = 2 needs a second CTA for such a token's three passes: 183 us.
+// 153 us, 4.4 TB/s, with the issue slots two thirds busy. kPasses = 3: such a token's three passes in one CTA.
 template <typename T, int D, bool INTERLEAVED, int H>
 __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendParams p) {
     constexpr int LANES = D / (2 * H), ROWS = 256 / LANES;
@@ -400,7 +400,7 @@ diopiError_t diopiB200RopeQuantAppendKV(diopiContextHandle_t ctx, diopiTensorHan
     }
     if (diopiError_t e = one_device(name, {q_out, qkv, cos, sin, positions, k_cache, k_scale, v_cache, v_scale}); e != diopiSuccess) return e;
     if (vx.numel == 0 || L == 0) return diopiSuccess;
-    B200_CHECK(vk.data != vv.data && vks.data != vvs.data, "%s: k and v must have caches and scales of their own", name);
+    B200_CHECK(vk.numel == 0 || (vk.data != vv.data && vks.data != vvs.data), "%s: k and v must have caches and scales of their own", name);
     B200_CHECK(B * S < 0x7fffffffLL && Hq + 2 * Hkv < 65536, "%s: too many tokens or heads", name);
     AppendParams p = {};
     p.qkv = vx.data; p.x_sb = vx.stride[0]; p.x_ss = tokens ? vx.stride[1] : 0;
