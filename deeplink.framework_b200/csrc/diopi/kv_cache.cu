@@ -57,7 +57,8 @@ __device__ __forceinline__ float max_abs8(float2 a, float2 b, float2 c, float2 d
 // The codes of 8 values, four to a word. amax: the row's largest magnitude, NaN if it holds one.
 __device__ __forceinline__ uint2 quantise(const float2 (&y)[4], float amax, float scale) {
     uint32_t code[8];
-    if (amax > 1e-30f && amax < INFINITY) {
+    // The fast division gives 0 for a divisor above 2^126.
+    if (amax > 1e-30f && amax < 0x1p126f) {
         // y * (127 / max|y|) + 1.5 * 2^23, rounded once to nearest even: the low byte of the sum is the code. Where the product is
         // within 2^-12 of a tie (it is within 127 * 2^-20 of the quotient) the quotient decides: a row's values are few bits long,
         // so half of the largest one, code 63.5, is no rare value.
@@ -87,7 +88,8 @@ __device__ __forceinline__ uint2 quantise(const float2 (&y)[4], float amax, floa
             }
         }
     } else {
-        // rows so small that 127 / max|y| may overflow, rows of zeros (also those whose scale underflows to zero), rows that are not finite
+        // rows so small or so large that 127 / max|y| leaves its range, rows of zeros (also those whose scale underflows to zero), rows that
+        // are not finite
         const bool zero = !(amax < INFINITY) || scale == 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
