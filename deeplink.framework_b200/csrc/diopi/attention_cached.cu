@@ -48,7 +48,7 @@ constexpr int64_t kWholeKeys = 512;
 // of one 99 against 95, 64 of 55 pieces 67 against 40).
 constexpr int64_t kWarpRows = 2048;
 constexpr float kLowest = -3e38f;    // a running maximum before the first score: finite, so that no difference with it is NaN
-constexpr float kGrow = 8.f;         // the running maximum follows only when a score outgrows it by this (log2): P stays below 2^8
+constexpr float kGrow = 8.f;         // the running maximum follows only when a score outgrows it by this (log2)
 
 struct CachedAttnParams {
     const void* q;
@@ -74,6 +74,22 @@ struct CachedAttnParams {
     float2* part_ml;               // the same slots' running maximum (log2) and sum
     PrefixParts prefix;            // splits = 0: no prefix
 };
+
+// Over int8 rows the second operand of O^T is P = e vs gain, e = 2^(s - m) <= 1, vs the row's scale: fp16, whose range is small beside
+// that of e vs. So every query head has a gain of its own, a power of two that has taken the largest e vs so far to [2^6, 2^7) and
+// follows when P outgrows kTop: a key without weight, whatever its scale, and a key of large weight and small scale leave the
+// others their bits. Below 2^-31 of the largest e vs a product has lost all of them. O is divided by the gain at the end.
+constexpr float kTop = 32768.f;
+__device__ __forceinline__ float gain_of(float largest) {     // finite, not negative
+    const int e = max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -120);
+    return __uint_as_float(static_cast<uint32_t>(127 + 6 - e) << 23);
+}
+__device__ __forceinline__ float inverse(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }   // of a power of two
+// What 2^6 stands for under a gain, after the running maximum has taken the products down by f.
+__device__ __forceinline__ float held(float gain, float f) { return f * (64.f * inverse(gain)); }
+// From one gain to the next, with the running maximum's factor.
+__device__ __forceinline__ float step(float from, float to, float f) { return f * to * inverse(from); }
+__device__ __forceinline__ float finite_or_zero(float x) { return x < INFINITY ? x : 0.f; }
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -190,6 +206,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
     constexpr int KS = D / 16;                                    // contraction steps of S^T = tiles of 16 columns of O
     constexpr int NQ = 8 * NT;
     constexpr int ES = QUANT ? 1 : 2;
+    constexpr float LIFT = QUANT ? -kGrow : 0.f;                  // m is the running maximum less this: e <= 2^(kGrow + LIFT)
     // P in the operand type is as coarse as the result, except for bf16 results over int8 rows, whose P is fp16. There it takes two
     // terms, P rounded and what the rounding left, in two products: the tensor cores have the time.
     constexpr int TERMS = QUANT && std::is_same<T, bf16>::value ? 1 : 2;
@@ -425,10 +442,11 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
         }
 
         float m[NT][2], l[NT][2], acc[NT][KS][4];
-        float vref = 0.f, ivref = 0.f;   // QUANT: P is held relative to the largest value scale so far (rounded up to a power of two)
+        float gain[NT][2];               // QUANT
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = kLowest;
+            gain[nt][0] = gain[nt][1] = 1.f;
             l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
@@ -488,8 +506,12 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                 }
                 bool grow = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) grow |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + kGrow || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + kGrow;
-                if (__any_sync(0xffffffffu, grow)) {
+                for (int nt = 0; nt < NT; ++nt) grow |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + (kGrow + LIFT) || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + (kGrow + LIFT);
+                grow = __any_sync(0xffffffffu, grow);
+                float f[NT][2];     // what the growth of the maxima takes older probabilities down by
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) f[nt][0] = f[nt][1] = 1.f;
+                if (grow) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -498,44 +520,72 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                            x = fmaxf(x, m[nt][c]);
-                            const float f = exp2_approx(m[nt][c] - x);
+                            x = fmaxf(x - LIFT, m[nt][c]);
+                            f[nt][c] = exp2_approx(m[nt][c] - x);
                             m[nt][c] = x;
-                            l[nt][c] *= f;
+                            l[nt][c] *= f[nt][c];
+                            if constexpr (!QUANT) {
 #pragma unroll
-                            for (int i = 0; i < KS; ++i) {
-                                acc[nt][i][c] *= f;
-                                acc[nt][i][2 + c] *= f;
+                                for (int i = 0; i < KS; ++i) {
+                                    acc[nt][i][c] *= f[nt][c];
+                                    acc[nt][i][2 + c] *= f[nt][c];
+                                }
                             }
                         }
                     }
                 }
-                if (QUANT) {
-                    const uint32_t vm = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(vs0), fabsf(vs1))));
-                    if (vm > __float_as_uint(vref) && vm < 0x7f000000u) {
-                        const float up = __uint_as_float((vm & 0x7f800000u) + 0x00800000u);
-                        ivref = 1.f / up;
-                        const float f = vref * ivref;
-                        vref = up;
+                float e[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        e[nt][c] = exp2_approx(s[nt][c] - m[nt][c]);
+                        e[nt][2 + c] = exp2_approx(s[nt][2 + c] - m[nt][c]);
+                        l[nt][c] += e[nt][c] + e[nt][2 + c];
+                    }
+                }
+                if constexpr (QUANT) {
+                    bool over = false;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            e[nt][c] *= vs0;
+                            e[nt][2 + c] *= vs1;
+                            over |= fmaxf(fabsf(e[nt][c]), fabsf(e[nt][2 + c])) * gain[nt][c] > kTop;
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, over) || grow) {
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                            for (int i = 0; i < KS; ++i) {
-                                acc[nt][i][0] *= f; acc[nt][i][1] *= f;
-                                acc[nt][i][2] *= f; acc[nt][i][3] *= f;
+                            for (int c = 0; c < 2; ++c) {
+                                float x = fmaxf(finite_or_zero(fabsf(e[nt][c])), finite_or_zero(fabsf(e[nt][2 + c])));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                                const float to = gain_of(fmaxf(x, held(gain[nt][c], f[nt][c]))), k = step(gain[nt][c], to, f[nt][c]);
+                                gain[nt][c] = to;
+#pragma unroll
+                                for (int i = 0; i < KS; ++i) {
+                                    acc[nt][i][c] *= k;
+                                    acc[nt][i][2 + c] *= k;
+                                }
                             }
                         }
                     }
-                    vs0 *= ivref;
-                    vs1 *= ivref;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            e[nt][c] *= gain[nt][c];
+                            e[nt][2 + c] *= gain[nt][c];
+                        }
+                    }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const float e0 = exp2_approx(s[nt][0] - m[nt][0]), e1 = exp2_approx(s[nt][1] - m[nt][1]);
-                    const float e2 = exp2_approx(s[nt][2] - m[nt][0]), e3 = exp2_approx(s[nt][3] - m[nt][1]);
-                    l[nt][0] += e0 + e2;
-                    l[nt][1] += e1 + e3;
-                    float2 lo = make_float2(e0 * vs0, e1 * vs0), hi = make_float2(e2 * vs1, e3 * vs1);   // keys g, g + 8
+                    float2 lo = make_float2(e[nt][0], e[nt][1]), hi = make_float2(e[nt][2], e[nt][3]);   // keys g, g + 8
 #pragma unroll
                     for (int k = 0; k < TERMS; ++k) {
                         const uint32_t a = Pair<M>::narrow(lo), c = Pair<M>::narrow(hi);
@@ -597,7 +647,6 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
 
         if (at.left > 0) load_queries();
         // ---- join the four warps: 2 and 3 into 0 and 1, then 1 into 0. A lane's values meet the same lane's ----
-        if (!QUANT) vref = 1.f;
         auto put_slot = [&](float* slot) {
             float4* d = reinterpret_cast<float4*>(slot) + lane;
 #pragma unroll
@@ -606,29 +655,35 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                 for (int i = 0; i < KS; ++i) d[(nt * (KS + 1) + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
                 d[(nt * (KS + 1) + KS) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
             }
-            d[NT * (KS + 1) * 32] = make_float4(vref, 0.f, 0.f, 0.f);
+            if constexpr (QUANT) d[NT * (KS + 1) * 32] = make_float4(gain[0][0], gain[0][1], gain[NT - 1][0], gain[NT - 1][1]);
         };
         auto add_slot = [&](const float* slot) {
             const float4* d = reinterpret_cast<const float4*>(slot) + lane;
-            const float ref = d[NT * (KS + 1) * 32].x, top = fmaxf(vref, ref);
-            const float ra = top > 0.f ? vref / top : 0.f, rb = top > 0.f ? ref / top : 0.f;
-            vref = top;
+            const float4 gains = QUANT ? d[NT * (KS + 1) * 32] : make_float4(1.f, 1.f, 1.f, 1.f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float4 x = d[(nt * (KS + 1) + KS) * 32];
                 const float m0 = fmaxf(m[nt][0], x.x), m1 = fmaxf(m[nt][1], x.y);
-                const float fa0 = exp2_approx(m[nt][0] - m0), fa1 = exp2_approx(m[nt][1] - m1), fb0 = exp2_approx(x.x - m0), fb1 = exp2_approx(x.y - m1);
+                float fa0 = exp2_approx(m[nt][0] - m0), fa1 = exp2_approx(m[nt][1] - m1), fb0 = exp2_approx(x.x - m0), fb1 = exp2_approx(x.y - m1);
                 l[nt][0] = l[nt][0] * fa0 + x.z * fb0;
                 l[nt][1] = l[nt][1] * fa1 + x.w * fb1;
                 m[nt][0] = m0;
                 m[nt][1] = m1;
+                if constexpr (QUANT) {
+                    const float g0 = nt == 0 ? gains.x : gains.z, g1 = nt == 0 ? gains.y : gains.w;
+                    const float to0 = gain_of(fmaxf(held(gain[nt][0], fa0), held(g0, fb0))), to1 = gain_of(fmaxf(held(gain[nt][1], fa1), held(g1, fb1)));
+                    fa0 = step(gain[nt][0], to0, fa0); fb0 = step(g0, to0, fb0);
+                    fa1 = step(gain[nt][1], to1, fa1); fb1 = step(g1, to1, fb1);
+                    gain[nt][0] = to0;
+                    gain[nt][1] = to1;
+                }
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
                     const float4 o = d[(nt * (KS + 1) + i) * 32];
-                    acc[nt][i][0] = acc[nt][i][0] * (fa0 * ra) + o.x * (fb0 * rb);
-                    acc[nt][i][1] = acc[nt][i][1] * (fa1 * ra) + o.y * (fb1 * rb);
-                    acc[nt][i][2] = acc[nt][i][2] * (fa0 * ra) + o.z * (fb0 * rb);
-                    acc[nt][i][3] = acc[nt][i][3] * (fa1 * ra) + o.w * (fb1 * rb);
+                    acc[nt][i][0] = acc[nt][i][0] * fa0 + o.x * fb0;
+                    acc[nt][i][1] = acc[nt][i][1] * fa1 + o.y * fb1;
+                    acc[nt][i][2] = acc[nt][i][2] * fa0 + o.z * fb0;
+                    acc[nt][i][3] = acc[nt][i][3] * fa1 + o.w * fb1;
                 }
             }
         };
@@ -664,9 +719,10 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                     ll += __shfl_xor_sync(0xffffffffu, ll, 16);
                     const int q = nt * 8 + 2 * t + c;
                     if (q >= rows) continue;
+                    const float back = QUANT ? inverse(gain[nt][c]) : 1.f;
                     // a lane holds runs of 8 (int8 rows of 128: 16) neighbouring columns
                     if (last_word) {
-                        const float f = ll == 0.f ? 0.f : vref / ll;
+                        const float f = ll == 0.f ? 0.f : back / ll;
                         T* dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(row0 + q) * p.o_sh;
 #pragma unroll
                         for (int i = 0; i < KS; i += 4) {
@@ -682,7 +738,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
 #pragma unroll
                         for (int i = 0; i < KS; i += 2) {
                             *reinterpret_cast<float4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 + (2 * i & 7) : g * KS * 2 + 2 * i)) =
-                                make_float4(acc[nt][i][c] * vref, acc[nt][i][2 + c] * vref, acc[nt][i + 1][c] * vref, acc[nt][i + 1][2 + c] * vref);
+                                make_float4(acc[nt][i][c] * back, acc[nt][i][2 + c] * back, acc[nt][i + 1][c] * back, acc[nt][i + 1][2 + c] * back);
                         }
                         if (g == 0) p.part_ml[slot * NQ + q] = make_float2(m[nt][c], ll);
                     }
