@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
     constexpr int KS = D / 16;                                    // contraction steps of S^T = tiles of 16 columns of O
     constexpr int NQ = 8 * NT;
     constexpr int ES = QUANT ? 1 : 2;
-    constexpr float LIFT = QUANT ? -kGrow : 0.f;                  // m is the running maximum less this: e <= 2^(kGrow + LIFT)
+    // m is the running maximum less this, so e <= 2^(kGrow + LIFT): fp16 keeps probabilities down to 2^-31 of the largest one that way.
+    constexpr float LIFT = QUANT ? -kGrow : (std::is_same<T, fp16>::value ? 7.f : 0.f);
     // P in the operand type is as coarse as the result, except for bf16 results over int8 rows, whose P is fp16. There it takes two
     // terms, P rounded and what the rounding left, in two products: the tensor cores have the time.
     constexpr int TERMS = QUANT && std::is_same<T, bf16>::value ? 1 : 2;

@@ -6,7 +6,7 @@ held for the second product
   over int8 rows              as fp16, its products p vs lifted so that a column's largest one lies at 2^6 or more: relative 2^-11 (bf16
                               results), 2^-22 (fp16 results: two terms), and 2^-25 / 2^6 of the largest product where it is subnormal
   over rows in bf16           in two terms, 2^-16, bf16 having fp32's range
-  over rows in fp16           in two terms, 2^-22, and 2^-25 of the largest probability
+  over rows in fp16           in two terms, 2^-22, the largest one lifted to 2^7: 2^-25 / 2^7 of the largest probability
   over a shared prompt        in one term, 2^-8 (bf16) or 2^-11 (fp16, and 2^-25 of the largest probability).
 Scores carry the fp32 sums' D 2^-24 relative to S = scale sum |q k|, in numerator and denominator, exponentials and sums 2^-20; the
 second product's fp32 sums 2^-22 A for each of a warp's n / 16 steps and the 64 of the joins; the result is rounded once.
@@ -110,7 +110,7 @@ def _hold(pkg, ctx, q, cache, lengths, scale, prefix=None, sequences=None):
                 if quant:
                     tol = tol + n * 2.0 ** -31 * 127 * (po * cache[3][b, h, :n].double().abs()).amax(-1, keepdim=True)
                 elif dtype is FP:
-                    tol = tol + n * 2.0 ** -25 * po.amax(-1, keepdim=True) * vo.abs().amax(0)
+                    tol = tol + n * 2.0 ** -32 * po.amax(-1, keepdim=True) * vo.abs().amax(0)
             err = (out[b, h * g:(h + 1) * g].double() - want).abs()
             assert (err <= tol).all(), (b, h, n, (err / tol).max().item())
             lerr = (lse[b, h * g:(h + 1) * g].double() - wlse).abs()
@@ -178,7 +178,7 @@ def _sink_case(quant, dtype, n, nats, at, vscale, D=128):
     return q, cache, [n], scale
 
 
-@pytest.mark.parametrize("quant,dtype", KINDS[:3])
+@pytest.mark.parametrize("quant,dtype", KINDS)
 @pytest.mark.parametrize("at", [0, 1500, 2900])
 @pytest.mark.parametrize("nats", [12.0, 15.0])
 def test_many_keys_behind_sink_keys(pkg, ctx, quant, dtype, at, nats):
