@@ -38,7 +38,7 @@ constexpr int kBlock = 128;            // keys per block
 constexpr int kRing = 3;
 constexpr int kHalf = 128 * 128;       // 128 rows of 128 bytes (64 two-byte columns), 128-byte swizzle
 constexpr int kPBytes = 2 * kHalf;     // P tile: 128 x 128 two-byte
-constexpr float kRescale = 8.f;        // log2 units: P stays below 2^8
+constexpr float kRescale = 8.f;        // log2 units: the running maximum follows when a score outgrows it by this
 
 template <int D>
 struct Smem {
@@ -222,6 +222,9 @@ __global__ void __launch_bounds__(384, 1) prefix_attention_kernel(const __grid_c
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t s_tmem = lane_base + t * 128, o_tmem = lane_base + 256 + t * 128;
         bool ok = true;
+        // m_used is the running maximum less this, so P stays below 2^(kRescale + LIFT): fp16 keeps probabilities down to 2^-31 of the
+        // largest one that way.
+        constexpr float LIFT = std::is_same<T, fp16>::value ? 7.f : 0.f;
         int done = 0, turns = 0;   // blocks of this tile, and blocks that both tiles have, of the segments before
         for (int x = x0; x < x1 && ok;) {
             const Segment g = segment(x);
@@ -278,11 +281,11 @@ __global__ void __launch_bounds__(384, 1) prefix_attention_kernel(const __grid_c
                 bool rescale = false;
                 float factor = 1.f;
                 if (j == 0) {
-                    m_used = mx;
+                    m_used = mx - LIFT;
                 } else {
-                    rescale = __any_sync(0xffffffffu, mx > m_used + kRescale);
+                    rescale = __any_sync(0xffffffffu, mx > m_used + (kRescale + LIFT));
                     if (rescale) {
-                        const float m_new = fmaxf(m_used, mx);
+                        const float m_new = fmaxf(m_used, mx - LIFT);
                         factor = (m_used == -INFINITY) ? 0.f : exp2_approx(m_used - m_new);
                         m_used = m_new;
                         l_sum *= factor;

@@ -7,7 +7,7 @@ held for the second product
                               results), 2^-22 (fp16 results: two terms), and 2^-25 / 2^6 of the largest product where it is subnormal
   over rows in bf16           in two terms, 2^-16, bf16 having fp32's range
   over rows in fp16           in two terms, 2^-22, the largest one lifted to 2^7: 2^-25 / 2^7 of the largest probability
-  over a shared prompt        in one term, 2^-8 (bf16) or 2^-11 (fp16, and 2^-25 of the largest probability).
+  over a shared prompt        in one term, 2^-8 (bf16) or 2^-11 (fp16, and 2^-32 of the largest probability).
 Scores carry the fp32 sums' D 2^-24 relative to S = scale sum |q k|, in numerator and denominator, exponentials and sums 2^-20; the
 second product's fp32 sums 2^-22 A for each of a warp's n / 16 steps and the 64 of the joins; the result is rounded once.
 """
@@ -102,7 +102,7 @@ def _hold(pkg, ctx, q, cache, lengths, scale, prefix=None, sequences=None):
             if P:
                 tol = tol + HALF[dtype] * (p[:, :P] @ v[:P].abs())
                 if dtype is FP:
-                    tol = tol + P * 2.0 ** -25 * p[:, :P].amax(-1, keepdim=True) * v[:P].abs().amax(0)
+                    tol = tol + P * 2.0 ** -32 * p[:, :P].amax(-1, keepdim=True) * v[:P].abs().amax(0)
             if n:
                 po, vo = p[:, P:], v[P:]
                 two = dtype is FP or not quant
@@ -237,3 +237,16 @@ def test_value_magnitudes_that_grow_and_fall(pkg, ctx):
             ramp = torch.logspace(-3, 3, 700, device=DEV)
             cache[3] *= ramp.flip(0) if flip else ramp
             _hold(pkg, ctx, _randn((2, 4, 64), 1, dtype).to(DEV), cache, [700, 401], 0.125)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("at", [0, 700, 1499])
+def test_many_prompt_rows_behind_a_sink_row(pkg, ctx, dtype, at):
+    """160 key heads, so that a CTA takes all rows of one, or most of them."""
+    H = 160
+    q, cache, _, scale = _sink_case(False, dtype, 1500, 15.0, [at], 1e-3)
+    prefix = [t[0, 0, :, None].expand(1500, H, 128).contiguous() for t in (cache[0], cache[2])]
+    own = _cache(True, dtype, 1, 1, 40, 128)
+    own[0].zero_()
+    for n in (0, 40):
+        _hold(pkg, ctx, q.expand(1, H, 128), [t.expand(1, H, *t.shape[2:]) for t in own], [n], scale, prefix)
