@@ -62,6 +62,9 @@ struct CachedAttnParams {
     int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl, ks_sb, ks_sh, vs_sb, vs_sh;   // elements
     const int64_t* lengths;
     int64_t L;
+    const void* pk;                // the shared prompt's rows, P of them
+    const void* pv;
+    int64_t pk_sp, pk_sh, pv_sp, pv_sh, P;
     int B, Hq, Hkv, group;
     int tiles;                     // groups of 8 NT query heads per key head
     int whole;                     // 1: a CTA takes whole segments, nothing is joined
@@ -195,8 +198,48 @@ struct Cursor {
     }
 };
 
+// Writes the values of out's row (b, h) again that are not finite although the row's softmax is (lse2: log2 of its denominator). Where an
+// infinity stands among the values, a probability in two terms, one that rounds to zero and the copies that fill a short tile give
+// inf - inf or 0 * inf; where values near the type's largest are summed before they are divided, the sum may leave fp32. Here the
+// divided probabilities, positive for every score above -inf, meet the values one key after the other. One warp; rare, and not fast.
+template <typename T, int D>
+__device__ __noinline__ void redo_row(const CachedAttnParams& p, int b, int h, float lse2) {
+    constexpr int N = D / 32;
+    const int at = (threadIdx.x & 31) * N, hk = h / p.group;
+    T* const dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * p.o_sh + at;
+    const T* const src = static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(h) * p.q_sh + at;
+    float q[N], o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        q[i] = to_f32(src[i]);
+        o[i] = 0.f;
+    }
+    auto add = [&](const auto* k, const auto* v, float ks, float vs) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s = fmaf(q[i], to_f32(k[i]), s);
+        s = warp_sum(s) * (ks * p.scale_log2);
+        const float e = s == -INFINITY ? 0.f : fmaxf(exp2_approx(s - lse2), 0x1p-126f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(e, to_f32(v[i]) * vs, o[i]);
+    };
+    for (int64_t i = 0; i < p.P; ++i)
+        add(static_cast<const T*>(p.pk) + i * p.pk_sp + hk * p.pk_sh + at, static_cast<const T*>(p.pv) + i * p.pv_sp + hk * p.pv_sh + at, 1.f, 1.f);
+    const int64_t n = p.own ? min(max(p.lengths[b], int64_t(0)), p.L) : 0, k0 = b * p.k_sb + hk * p.k_sh + at, v0 = b * p.v_sb + hk * p.v_sh + at;
+    for (int64_t i = 0; i < n; ++i) {
+        if (p.ks != nullptr)
+            add(static_cast<const int8_t*>(p.k) + k0 + i * p.k_sl, static_cast<const int8_t*>(p.v) + v0 + i * p.v_sl, p.ks[b * p.ks_sb + hk * p.ks_sh + i], p.vs[b * p.vs_sb + hk * p.vs_sh + i]);
+        else
+            add(static_cast<const T*>(p.k) + k0 + i * p.k_sl, static_cast<const T*>(p.v) + v0 + i * p.v_sl, 1.f, 1.f);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (!(fabsf(to_f32(dst[i])) < INFINITY)) dst[i] = from_f32<T>(o[i]);
+    }
+}
+
 template <typename T, bool QUANT, int D, int NT>
-__global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attention_kernel(const CachedAttnParams p) {
+__global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attention_kernel(const __grid_constant__ CachedAttnParams p) {
     using M = typename std::conditional<QUANT, fp16, T>::type;    // operand type of the products
     using R = Ring<QUANT, D, NT>;
     constexpr int ROW = R::kRow;
@@ -709,6 +752,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
             add_slot(slot1);
             if (at.left > 0) barrier_arrive(kTaken3);
             const bool last_word = complete && p.prefix.splits == 0;
+            uint32_t again = 0;       // columns to be redone
             const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + static_cast<int64_t>(b) * W + hw : 2 * static_cast<int64_t>(blockIdx.x) + (from_start ? 1 : 0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -725,15 +769,22 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                     if (last_word) {
                         const float f = ll == 0.f ? 0.f : back / ll;
                         T* dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(row0 + q) * p.o_sh;
+                        float sum = 0.f;
 #pragma unroll
                         for (int i = 0; i < KS; i += 4) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) w[j] = Pair<T>::narrow(make_float2(acc[nt][i + j][c] * f, acc[nt][i + j][2 + c] * f));
+                            for (int j = 0; j < 4; ++j) {
+                                const float2 x = make_float2(acc[nt][i + j][c] * f, acc[nt][i + j][2 + c] * f);
+                                w[j] = Pair<T>::narrow(x);
+                                sum += x.x + x.y;
+                            }
                             *reinterpret_cast<uint4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 : g * KS * 2 + 2 * i)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
+                        l[nt][c] = m[nt][c] + log2f(ll);
+                        if (!(fabsf(sum) < INFINITY) && ll > 0.f) again |= 1u << (2 * nt + c);
                         if (g == 0 && p.lse != nullptr)
-                            p.lse[b * p.lse_sb + static_cast<int64_t>(row0 + q) * p.lse_sh] = ll == 0.f ? -INFINITY : (m[nt][c] + log2f(ll)) * 0.6931471805599453f;
+                            p.lse[b * p.lse_sb + static_cast<int64_t>(row0 + q) * p.lse_sh] = ll == 0.f ? -INFINITY : l[nt][c] * 0.6931471805599453f;
                     } else {
                         float* dst = p.part_o + (slot * NQ + q) * D;
 #pragma unroll
@@ -742,6 +793,19 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                                 make_float4(acc[nt][i][c] * back, acc[nt][i][2 + c] * back, acc[nt][i + 1][c] * back, acc[nt][i + 1][2 + c] * back);
                         }
                         if (g == 0) p.part_ml[slot * NQ + q] = make_float2(m[nt][c], ll);
+                    }
+                }
+            }
+            if (last_word && __any_sync(0xffffffffu, again != 0)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t lanes = __ballot_sync(0xffffffffu, (again >> (2 * nt + c)) & 1);
+                        for (int j = 0; j < 4; ++j) {
+                            const float x = __shfl_sync(0xffffffffu, l[nt][c], j);
+                            if (lanes & (0x11111111u << j)) redo_row<T, D>(p, b, row0 + nt * 8 + 2 * j + c, x);
+                        }
                     }
                 }
             }
@@ -755,7 +819,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
 // row: a CTA's sixteen where rows are few and have many pieces, one where rows are many. A warp keeps a running maximum over its
 // pieces, so that maxima and outputs are fetched together.
 template <typename T, int D, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attention_join_kernel(const CachedAttnParams p, int nq) {
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attention_join_kernel(const __grid_constant__ CachedAttnParams p, int nq) {
     constexpr int N = D / 32;
     __shared__ float sh_m[WARPS], sh_l[WARPS];
     __shared__ float sh_o[WARPS][D];
@@ -841,8 +905,14 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attentio
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * p.o_sh) + lane * (N / 2);
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) dst[i / 2] = Pair<T>::narrow(make_float2(o[i] * inv, o[i + 1] * inv));
+    for (int i = 0; i < N; i += 2) {
+        const float2 x = make_float2(o[i] * inv, o[i + 1] * inv);
+        dst[i / 2] = Pair<T>::narrow(x);
+        sum += x.x + x.y;
+    }
+    if (__any_sync(0xffffffffu, !(fabsf(sum) < INFINITY)) && l > 0.f) redo_row<T, D>(p, b, h, m + log2f(l));
     if (lane == 0 && p.lse != nullptr) p.lse[b * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
@@ -964,6 +1034,8 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     p.max_ctas = static_cast<int>(wanted < resident ? (wanted < 1 ? 1 : wanted) : resident);
     cudaStream_t stream = stream_of(ctx);
     if (P > 0) {
+        p.pk = vpk.data; p.pv = vpv.data; p.P = P;
+        p.pk_sp = vpk.stride[0]; p.pk_sh = vpk.stride[1]; p.pv_sp = vpv.stride[0]; p.pv_sh = vpv.stride[1];
         const diopiError_t e = prefix_attention(name, ctx, vq, vpk, vpv, p.scale_log2, &p.prefix, stream);
         if (e != diopiSuccess) return e;
     }

@@ -1,5 +1,5 @@
 """The ends of the value range in the operators on key / value caches: rows near the largest bf16, probabilities far below the
-largest one, value rows of very different magnitudes.
+largest one, value rows of very different magnitudes, infinities among the values.
 
 Tolerance of the attention (u = eps / 2, half a step of a type; p the exact softmax, A = sum p |v|, n the keys of a part). A probability is
 held for the second product
@@ -250,3 +250,68 @@ def test_many_prompt_rows_behind_a_sink_row(pkg, ctx, dtype, at):
     own[0].zero_()
     for n in (0, 40):
         _hold(pkg, ctx, q.expand(1, H, 128), [t.expand(1, H, *t.shape[2:]) for t in own], [n], scale, prefix)
+
+
+# ---- infinities among the values ----------------------------------------------------------------------------------------------------
+def _same(out, want):
+    """Infinities and NaN where the definition has them; the rest is the other tests' business."""
+    assert torch.equal(out.isnan(), want.isnan()), (int(out.isnan().sum()), int(want.isnan().sum()))
+    assert torch.equal(out.double().nan_to_num(0, 1e300, -1e300).abs() == 1e300, want.nan_to_num(0, 1e300, -1e300).abs() == 1e300)
+    inf = want.isinf()
+    assert torch.equal(out[inf].double(), want[inf])
+    err = (out[~inf & ~want.isnan()].double() - want[~inf & ~want.isnan()]).abs()
+    assert (err <= 0.02 * (1 + want[~inf & ~want.isnan()].abs())).all()
+
+
+@pytest.mark.parametrize("quant,dtype", KINDS)
+@pytest.mark.parametrize("L", [130, 700])
+@pytest.mark.parametrize("P", [0, 150])
+def test_infinite_values(pkg, ctx, quant, dtype, L, P):
+    """An infinity in a visible value row gives an infinity of its sign (NaN beside one of the other sign), also at the last key of a
+    ragged sequence and at a key of hardly any weight; one behind the sequence gives nothing."""
+    B, Hq, Hkv, D = 3, 6, 2, 128
+    q = _randn((B, Hq, D), 1, dtype).to(DEV)
+    cache = _cache(quant, dtype, B, Hkv, L, D)
+    lengths = [L, 77, 3]
+    if quant:
+        cache[3] *= 0.2
+        cache[3][0, 0, 5] = math.inf
+        cache[3][1, 1, 76] = math.inf
+        cache[3][2, :, 3:] = math.inf
+    else:
+        v = cache[2]
+        v[0, 0, 5, 7] = v[0, 0, L - 1, 9] = math.inf
+        v[0, 0, 11, 20] = -math.inf
+        v[0, 1, 2, 3], v[0, 1, 60, 3] = math.inf, -math.inf
+        v[1, 0, 76, 1] = v[1, 1, 30, 2] = -math.inf
+        v[2, :, 3:] = math.inf
+        cache[0][1, 1, 30] = _towards(q[1, 3], -60.0, D ** -0.5).to(dtype)
+    prefix = None
+    if P:
+        prefix = [_randn((P, Hkv, D), 8 + i, dtype).to(DEV) for i in range(2)]
+        prefix[1][P - 1, 0, 40], prefix[1][3, 1, 50] = math.inf, -math.inf
+        prefix[0][3, 1] = _towards(q[2, 4], -60.0, D ** -0.5).to(dtype)
+    out, lse = _run(pkg, ctx, q, cache, lengths, D ** -0.5, prefix)
+    g = Hq // Hkv
+    for b in range(B):
+        for h in range(Hkv):
+            _, _, v, s = _exact(q, cache, b, h, lengths[b], D ** -0.5, prefix)
+            p = torch.softmax(s, -1)
+            want = (p[:, :, None] * v[None]).sum(1)
+            _same(out[b, h * g:(h + 1) * g], want)
+    assert lse.isfinite().all()
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("L", [300, 900])
+@pytest.mark.parametrize("P", [0, 150])
+def test_sums_of_values_near_the_largest_bf16(pkg, ctx, quant, L, P):
+    """Their sum leaves fp32 before it is divided; the result does not."""
+    cache = _cache(quant, BF, 2, 2, L, 128)
+    if quant:
+        cache[3].fill_(3.3e38 / 127)
+    else:
+        cache[2][:] = (cache[2].float().clamp(-3, 3) * 1.1e38).to(BF)
+    prefix = [_randn((P, 2, 128), 8 + i, BF).to(DEV) for i in range(2)] if P else None
+    out = _hold(pkg, ctx, _randn((2, 4, 128), 1, BF).to(DEV), cache, [L, L // 2], 128 ** -0.5, prefix)
+    assert out.isfinite().all()
