@@ -560,7 +560,8 @@ class DecoderLayer:
 
     def decode_cached(self, x, cache, positions, lengths, prefix=None, ctx=None):
         """One token per sequence, x [batch, hidden], at each sequence's own place: positions int64 [batch] (the slot that receives the
-        new key and value; negative: the sequence is idle), lengths int64 [batch] (positions + 1; 0 for idle ones)."""
+        new key and value; negative: the sequence is idle), lengths int64 [batch] (positions + 1; 0 for idle ones). The rows of idle
+        sequences, and of those whose position lies past the cache, are finite and mean nothing: their query is zero."""
         ctx = ctx or diopi.Context()
         self._cached_supported()
         b, d, hq, hk = x.shape[0], self.head_dim, self.heads, self.kv_heads
@@ -570,6 +571,7 @@ class DecoderLayer:
         qkv = self._linear(ctx, hn, wqkv)
         cos, sin = self._cached_tables(cache, prefix)
         q, av = self._empty(b, hq, d), self._empty(b, hq, d)
+        self._call(diopi.diopiZeroInp, ctx, q)   # the writer leaves rows of tokens without a slot as they are
         self._call(diopi.diopiB200RopeQuantAppendKV, ctx, q, qkv, cos, sin, positions, *cache.args, self.interleaved)
         if prefix is None:
             self._call(diopi.diopiB200CachedAttention, ctx, av, None, q, *cache.args, lengths, 1.0 / math.sqrt(d))
