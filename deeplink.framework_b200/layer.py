@@ -197,6 +197,7 @@ class DecoderLayer:
         self.attention_norm = put(weights["attention_norm"])
         self.ffn_norm = put(weights["ffn_norm"])
         self._tables = {}
+        self._angles = []  # cos / sin for the int8 cache's positions, the last one in use
         self._masks = {}
         self._keep = None  # while capturing a graph: every temporary, so that its memory stays reserved for replays
         self.launches = 0  # DIOPI calls issued (each is at least one kernel launch or device copy)
@@ -508,8 +509,16 @@ class DecoderLayer:
     # A prompt that the whole batch shares is passed as `prefix`: its rotated keys and its values, [P, local kv heads, D] in the
     # model's type (one sequence's prefill gives them, prefix_kv). The sequences' own slots then stand for positions P, P + 1, ...
     def _cached_tables(self, cache, prefix):
-        first = 0 if prefix is None else prefix[0].shape[0]
-        return self._tables_for(("cached", first, cache.capacity), torch.arange(first, first + cache.capacity))
+        return self._angle_rows(0 if prefix is None else prefix[0].shape[0], cache.capacity)
+
+    def _angle_rows(self, first, count):
+        """cos / sin of positions first .. first + count - 1: rows of one table from position 0 on. It at least doubles when it grows, and the
+        smaller ones stay, in all less than the last: launches in flight and captured graphs may still read them."""
+        have = self._angles[-1][0].shape[0] if self._angles else 0
+        if first + count > have:
+            self._angles.append(rope_tables(self.head_dim, torch.arange(max(first + count, 2 * have)), self.rope_base, self.device))
+        cos, sin = self._angles[-1]
+        return cos[first:first + count], sin[first:first + count]
 
     def _cached_supported(self):
         assert self.dtype in (torch.bfloat16, torch.float16) and self.head_dim in (64, 128), "the int8 cache serves bfloat16 / float16 and head dim 64 or 128"
@@ -521,7 +530,7 @@ class DecoderLayer:
         hn = self._like(x)
         self._call(diopi.diopiRMSNorm, ctx, hn, None, x, [self.hidden], self.attention_norm, None, self.eps)
         k, v = self._linear(ctx, hn, self.wk).view(n, hk, d), self._linear(ctx, hn, self.wv).view(n, hk, d)
-        cos, sin = self._tables_for(("prefill", n), torch.arange(n))
+        cos, sin = self._angle_rows(0, n)
         return self._rope(ctx, k, cos, sin), v
 
     def prefill_cached(self, x, batch, seq, cache, start=0, prefix=None, ctx=None):
