@@ -6,9 +6,10 @@ device, exactly the metadata DIPU's diopirt callbacks expose. Every diopiXxx fun
 a non-zero return code raises DiopiError carrying diopiGetLastErrorString().
 """
 import ctypes
-import glob
 import importlib.util
 import os
+import sysconfig
+import warnings
 
 import torch
 
@@ -18,14 +19,19 @@ _lib = _native.diopi
 _host = _native.host
 
 
-def _load_call():
-    """The extension module that fills the tensor handles in C++ (built when torch's and Python's headers are present)."""
-    paths = glob.glob(os.path.join(_native.LIB_DIR, "dipu_b200_call*.so"))
-    if not paths:
+def _load_call(lib_dir=_native.LIB_DIR):
+    """The extension module that fills the tensor handles in C++ (built when torch's and Python's headers are present), for this
+    interpreter. Without it, and with one that does not load (built against another torch), calls go through ctypes."""
+    path = os.path.join(lib_dir, "dipu_b200_call" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+    if not os.path.exists(path):
         return None
-    spec = importlib.util.spec_from_file_location("dipu_b200_call", paths[0])
-    mod = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(mod)
+    spec = importlib.util.spec_from_file_location("dipu_b200_call", path)
+    try:
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+    except ImportError as e:
+        warnings.warn("dipu_b200_call is left out, calls take longer on the host: %s" % e, RuntimeWarning)
+        return None
     return mod
 
 
