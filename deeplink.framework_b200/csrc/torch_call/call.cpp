@@ -131,7 +131,7 @@ PyObject* call(PyObject* self, PyObject* const* args, Py_ssize_t n) {
                 break;
             }
             default: {
-                PyObject* v = PyNumber_Long(x);
+                PyObject* v = PyNumber_Index(x);   // an integer of any kind; a fraction or a text is an error
                 if (v == nullptr) return nullptr;
                 a[na++] = static_cast<uint64_t>(PyLong_AsLongLong(v));
                 Py_DECREF(v);
