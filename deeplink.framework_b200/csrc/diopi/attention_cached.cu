@@ -22,6 +22,7 @@
 // under the exponent of 1024, minus 1152), 1.25 to 1.5 instructions a value. A tile costs a warp about 435 instructions; with that the
 // products take as long as the memory at 1.95 GHz, and longer below.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -979,7 +980,9 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     }
     B200_CHECK(vn.dtype == diopi_dtype_int64 && vn.ndim == 1 && vn.shape[0] == B && vn.is_contiguous() && vn.device == diopi_device,
                "%s: lengths must be a dense int64 tensor [batch] on the device", name);
+    const double scale_log2 = scale * 1.4426950408889634;
     B200_CHECK(std::isfinite(scale) && scale > 0.0, "%s: scale must be positive, got %g", name, scale);
+    B200_CHECK(scale_log2 >= FLT_MIN && scale_log2 <= FLT_MAX, "%s: scale leaves float32's range, got %g", name, scale);
     if (softmax_lse) {
         B200_CHECK(vl.dtype == diopi_dtype_float32 && vl.ndim == 2 && vl.shape[0] == B && vl.shape[1] == Hq && vl.device == diopi_device,
                    "%s: softmax_lse must be float32 [batch, heads]", name);
@@ -1027,7 +1030,7 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     p.tiles = static_cast<int>(tiles);
     p.own = L > 0 ? 1 : 0;
     p.whole = L <= kWholeKeys ? 1 : 0;
-    p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+    p.scale_log2 = static_cast<float>(scale_log2);
     const bool wide = vq.dtype == diopi_dtype_bfloat16;
     const int64_t resident = static_cast<int64_t>(sm_count()) * resident_ctas(D, k_scale != nullptr, nt);
     const int64_t wanted = p.whole ? segments : (most_places + kMinPlaces - 1) / kMinPlaces;
