@@ -63,9 +63,8 @@ struct CachedAttnParams {
     int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl, ks_sb, ks_sh, vs_sb, vs_sh;   // elements
     const int64_t* lengths;
     int64_t L;
-    const void* pk;                // the shared prompt's rows, P of them
-    const void* pv;
-    int64_t pk_sp, pk_sh, pv_sp, pv_sh, P;
+    const void* pv;                // the shared prompt's values, P rows
+    int64_t pv_sp, pv_sh, P;
     int B, Hq, Hkv, group;
     int tiles;                     // groups of 8 NT query heads per key head
     int whole;                     // 1: a CTA takes whole segments, nothing is joined
@@ -199,43 +198,62 @@ struct Cursor {
     }
 };
 
-// Writes the values of out's row (b, h) again that are not finite although the row's softmax is (lse2: log2 of its denominator). Where an
-// infinity stands among the values, a probability in two terms, one that rounds to zero and the copies that fill a short tile give
-// inf - inf or 0 * inf; where values near the type's largest are summed before they are divided, the sum may leave fp32. Here the
-// divided probabilities, positive for every score above -inf, meet the values one key after the other. One warp; rare, and not fast.
+// The infinities of out's row (b, h), where some of it is not finite although its softmax is. Probabilities are positive, so a column with
+// an infinity among its values is that infinity, or NaN beside one of the other sign or a NaN; but a probability in two terms, one
+// that rounds to zero and the copies that fill a short tile make it inf - inf or 0 * inf. So the values alone decide, taken down far enough
+// that finite ones stay finite. One warp, two rows at a time (more
+// registers here slow the join down), some 240 ns a row; it stops where NaN is all that can come out.
 template <typename T, int D>
-__device__ __noinline__ void redo_row(const CachedAttnParams& p, int b, int h, float lse2) {
-    constexpr int N = D / 32;
-    const int at = (threadIdx.x & 31) * N, hk = h / p.group;
+__device__ __noinline__ void settle_infinities(const CachedAttnParams& p, int b, int h) {
+    constexpr int N = D / 32, AT_ONCE = 2;
+    const int lane = threadIdx.x & 31, at = lane * N, hk = h / p.group;
     T* const dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * p.o_sh + at;
-    const T* const src = static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(h) * p.q_sh + at;
-    float q[N], o[N];
+    const int64_t n = p.own ? min(max(p.lengths[b], int64_t(0)), p.L) : 0;
+    const float* const scales = p.ks != nullptr ? p.vs + b * p.vs_sb + hk * p.vs_sh : nullptr;
+    __syncwarp();                     // other lanes wrote some of the row
+    if (scales != nullptr) {          // codes are finite: nothing to do beside a scale that is NaN, nor without one that is infinite
+        bool nan = false, inf = false;
+        for (int64_t i = lane; i < n; i += 32) {
+            nan |= isnan(scales[i]);
+            inf |= isinf(scales[i]);
+        }
+        if (__any_sync(0xffffffffu, nan) || (p.P == 0 && !__any_sync(0xffffffffu, inf))) return;
+    }
+    float o[N];
+    bool open[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        q[i] = to_f32(src[i]);
         o[i] = 0.f;
+        open[i] = !(fabsf(to_f32(dst[i])) < INFINITY);
     }
-    auto add = [&](const auto* k, const auto* v, float ks, float vs) {
-        float s = 0.f;
+    auto add = [&](const auto* v, int64_t pitch, const float* vs, int64_t count) {
+        for (int64_t j = 0; j < count; j += AT_ONCE) {
+            bool more = false;
+            typename std::remove_const<typename std::remove_pointer<decltype(v)>::type>::type x[AT_ONCE][N];
+            float f[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(q[i], to_f32(k[i]), s);
-        s = warp_sum(s) * (ks * p.scale_log2);
-        const float e = s == -INFINITY ? 0.f : fmaxf(exp2_approx(s - lse2), 0x1p-126f);
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int64_t r = min(j + u, count - 1);
+                memcpy(x[u], __builtin_assume_aligned(v + r * pitch, sizeof(x[u])), sizeof(x[u]));
+                f[u] = vs != nullptr ? vs[r] : 1.f;
+            }
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(e, to_f32(v[i]) * vs, o[i]);
+            for (int u = 0; u < AT_ONCE; ++u) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) o[i] = fmaf(to_f32(x[u][i]) * f[u], 0x1p-64f, o[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) more |= open[i] && !isnan(o[i]);
+            if (!__any_sync(0xffffffffu, more)) return;
+        }
     };
-    for (int64_t i = 0; i < p.P; ++i)
-        add(static_cast<const T*>(p.pk) + i * p.pk_sp + hk * p.pk_sh + at, static_cast<const T*>(p.pv) + i * p.pv_sp + hk * p.pv_sh + at, 1.f, 1.f);
-    const int64_t n = p.own ? min(max(p.lengths[b], int64_t(0)), p.L) : 0, k0 = b * p.k_sb + hk * p.k_sh + at, v0 = b * p.v_sb + hk * p.v_sh + at;
-    for (int64_t i = 0; i < n; ++i) {
-        if (p.ks != nullptr)
-            add(static_cast<const int8_t*>(p.k) + k0 + i * p.k_sl, static_cast<const int8_t*>(p.v) + v0 + i * p.v_sl, p.ks[b * p.ks_sb + hk * p.ks_sh + i], p.vs[b * p.vs_sb + hk * p.vs_sh + i]);
-        else
-            add(static_cast<const T*>(p.k) + k0 + i * p.k_sl, static_cast<const T*>(p.v) + v0 + i * p.v_sl, 1.f, 1.f);
-    }
+    if (p.P > 0) add(static_cast<const T*>(p.pv) + hk * p.pv_sh + at, p.pv_sp, nullptr, p.P);
+    const int64_t v0 = b * p.v_sb + hk * p.v_sh + at;
+    if (scales != nullptr) add(static_cast<const int8_t*>(p.v) + v0, p.v_sl, scales, n);
+    else add(static_cast<const T*>(p.v) + v0, p.v_sl, nullptr, n);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (!(fabsf(to_f32(dst[i])) < INFINITY)) dst[i] = from_f32<T>(o[i]);
+        if (open[i] && !(fabsf(o[i]) < INFINITY)) dst[i] = from_f32<T>(o[i]);
     }
 }
 
@@ -250,8 +268,9 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
     constexpr int KS = D / 16;                                    // contraction steps of S^T = tiles of 16 columns of O
     constexpr int NQ = 8 * NT;
     constexpr int ES = QUANT ? 1 : 2;
-    // m is the running maximum less this, so e <= 2^(kGrow + LIFT): fp16 keeps probabilities down to 2^-31 of the largest one that way.
-    constexpr float LIFT = QUANT ? -kGrow : (std::is_same<T, fp16>::value ? 7.f : 0.f);
+    // m is the running maximum less this, so e <= 2^(kGrow + LIFT). fp16 keeps probabilities down to 2^-31 of the largest one that way;
+    // the products with bf16 values, which may come near fp32's largest, and their sums stay in range.
+    constexpr float LIFT = QUANT ? -kGrow : (std::is_same<T, fp16>::value ? 7.f : -24.f);
     // P in the operand type is as coarse as the result, except for bf16 results over int8 rows, whose P is fp16. There it takes two
     // terms, P rounded and what the rounding left, in two products: the tensor cores have the time.
     constexpr int TERMS = QUANT && std::is_same<T, bf16>::value ? 1 : 2;
@@ -753,7 +772,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
             add_slot(slot1);
             if (at.left > 0) barrier_arrive(kTaken3);
             const bool last_word = complete && p.prefix.splits == 0;
-            uint32_t again = 0;       // columns to be redone
+            uint32_t settle = 0;      // query heads whose row is not finite
             const int64_t slot = complete ? (p.whole ? 0 : 2 * static_cast<int64_t>(p.max_ctas)) + static_cast<int64_t>(b) * W + hw : 2 * static_cast<int64_t>(blockIdx.x) + (from_start ? 1 : 0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -766,6 +785,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                     const int q = nt * 8 + 2 * t + c;
                     if (q >= rows) continue;
                     const float back = QUANT ? inverse(gain[nt][c]) : 1.f;
+                    constexpr float DOWN = QUANT ? 16.f : 0.f, BY = QUANT ? 0x1p-16f : 1.f;   // a piece of int8 rows takes the values' sums down, too
                     // a lane holds runs of 8 (int8 rows of 128: 16) neighbouring columns
                     if (last_word) {
                         const float f = ll == 0.f ? 0.f : back / ll;
@@ -782,32 +802,24 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                             }
                             *reinterpret_cast<uint4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 : g * KS * 2 + 2 * i)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                        l[nt][c] = m[nt][c] + log2f(ll);
-                        if (!(fabsf(sum) < INFINITY) && ll > 0.f) again |= 1u << (2 * nt + c);
+                        if (!(fabsf(sum) < INFINITY) && ll > 0.f) settle |= 1u << (2 * nt + c);
                         if (g == 0 && p.lse != nullptr)
-                            p.lse[b * p.lse_sb + static_cast<int64_t>(row0 + q) * p.lse_sh] = ll == 0.f ? -INFINITY : l[nt][c] * 0.6931471805599453f;
+                            p.lse[b * p.lse_sb + static_cast<int64_t>(row0 + q) * p.lse_sh] = ll == 0.f ? -INFINITY : (m[nt][c] + log2f(ll)) * 0.6931471805599453f;
                     } else {
                         float* dst = p.part_o + (slot * NQ + q) * D;
 #pragma unroll
                         for (int i = 0; i < KS; i += 2) {
                             *reinterpret_cast<float4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 + (2 * i & 7) : g * KS * 2 + 2 * i)) =
-                                make_float4(acc[nt][i][c] * back, acc[nt][i][2 + c] * back, acc[nt][i + 1][c] * back, acc[nt][i + 1][2 + c] * back);
+                                make_float4(acc[nt][i][c] * (back * BY), acc[nt][i][2 + c] * (back * BY), acc[nt][i + 1][c] * (back * BY), acc[nt][i + 1][2 + c] * (back * BY));
                         }
-                        if (g == 0) p.part_ml[slot * NQ + q] = make_float2(m[nt][c], ll);
+                        if (g == 0) p.part_ml[slot * NQ + q] = make_float2(m[nt][c] + DOWN, ll * BY);
                     }
                 }
             }
-            if (last_word && __any_sync(0xffffffffu, again != 0)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t lanes = __ballot_sync(0xffffffffu, (again >> (2 * nt + c)) & 1);
-                        for (int j = 0; j < 4; ++j) {
-                            const float x = __shfl_sync(0xffffffffu, l[nt][c], j);
-                            if (lanes & (0x11111111u << j)) redo_row<T, D>(p, b, row0 + nt * 8 + 2 * j + c, x);
-                        }
-                    }
+            if (last_word && __any_sync(0xffffffffu, settle != 0)) {
+                for (int q = 0; q < rows; ++q) {
+                    const uint32_t lanes = __ballot_sync(0xffffffffu, (settle >> (q / 8 * 2 + (q & 1))) & 1);
+                    if (lanes & (0x11111111u << ((q & 7) >> 1))) settle_infinities<T, D>(p, b, row0 + q);
                 }
             }
         }
@@ -913,7 +925,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attentio
         dst[i / 2] = Pair<T>::narrow(x);
         sum += x.x + x.y;
     }
-    if (__any_sync(0xffffffffu, !(fabsf(sum) < INFINITY)) && l > 0.f) redo_row<T, D>(p, b, h, m + log2f(l));
+    if (__any_sync(0xffffffffu, !(fabsf(sum) < INFINITY)) && l > 0.f) settle_infinities<T, D>(p, b, h);
     if (lane == 0 && p.lse != nullptr) p.lse[b * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
@@ -1037,8 +1049,7 @@ diopiError_t cached_attention(const char* name, diopiContextHandle_t ctx, diopiT
     p.max_ctas = static_cast<int>(wanted < resident ? (wanted < 1 ? 1 : wanted) : resident);
     cudaStream_t stream = stream_of(ctx);
     if (P > 0) {
-        p.pk = vpk.data; p.pv = vpv.data; p.P = P;
-        p.pk_sp = vpk.stride[0]; p.pk_sh = vpk.stride[1]; p.pv_sp = vpv.stride[0]; p.pv_sh = vpv.stride[1];
+        p.pv = vpv.data; p.pv_sp = vpv.stride[0]; p.pv_sh = vpv.stride[1]; p.P = P;
         const diopiError_t e = prefix_attention(name, ctx, vq, vpk, vpv, p.scale_log2, &p.prefix, stream);
         if (e != diopiSuccess) return e;
     }

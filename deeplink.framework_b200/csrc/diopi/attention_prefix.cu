@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(384, 1) prefix_attention_kernel(const __grid_c
         const uint32_t s_tmem = lane_base + t * 128, o_tmem = lane_base + 256 + t * 128;
         bool ok = true;
         // m_used is the running maximum less this, so P stays below 2^(kRescale + LIFT): fp16 keeps probabilities down to 2^-31 of the
-        // largest one that way.
-        constexpr float LIFT = std::is_same<T, fp16>::value ? 7.f : 0.f;
+        // largest one that way, and sums of bf16 values, which may come near fp32's largest, stay in range.
+        constexpr float LIFT = std::is_same<T, fp16>::value ? 7.f : -24.f;
         int done = 0, turns = 0;   // blocks of this tile, and blocks that both tiles have, of the segments before
         for (int x = x0; x < x1 && ok;) {
             const Segment g = segment(x);
