@@ -5,7 +5,7 @@
 //   diopiB200SharedPrefixAttention  the same over the rows of a prompt [P, Hkv, D], stored once, and then the sequence's own rows
 //
 // Bound by reading the cache: 2 (D + 4) bytes a key and key head (int8) against 4 D group flops. 64 sequences x 32 heads x 4096 keys x
-// 128: 2.22 GB in 348 us, 6.4 TB/s, as long as the clock holds; the card's power limit takes a steady loop to 1.65 GHz and 383 - 416 us.
+// 128: 2.22 GB in 364 us, 6.1 TB/s, in a single launch at 1.78 GHz; the card's power limit takes a steady loop to 1.65 GHz and 410 - 425 us.
 //
 // Work is cut evenly, whatever the lengths. A segment is one sequence x key head x group of up to 8 NT query heads; its keys count in
 // units of 64. The units of all segments, in order, are dealt to the CTAs in equal consecutive ranges, so a long sequence is spread
@@ -19,8 +19,11 @@
 // byte a larger instruction would not be filled; what this shape saves is the feeding, because the order of the contracted index is
 // free. For S^T a lane takes 16-byte chunks of its two key rows and the queries are laid out the same way; for O^T a lane takes 16
 // neighbouring columns of its four key rows and pairs of keys are zipped with byte permutes. int8 codes become fp16 exactly (a byte
-// under the exponent of 1024, minus 1152), 1.25 to 1.5 instructions a value. A tile costs a warp about 435 instructions; with that the
-// products take as long as the memory at 1.95 GHz, and longer below.
+// under the exponent of 1024, minus 1152), 1.25 to 1.5 instructions a value.
+//
+// A tile costs a warp about 430 instructions in one chain - scores, maximum, exponentials, transposition, values - that three warps a
+// scheduler do not hide: issue slots 60 % busy, the busiest pipe 52 %, waits for fixed latencies the largest stall. 8 % fewer instructions
+// took 411 us against 413; the copies without the products take 347 at any clock.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -201,8 +204,8 @@ struct Cursor {
 // The infinities of out's row (b, h), where some of it is not finite although its softmax is. Probabilities are positive, so a column with
 // an infinity among its values is that infinity, or NaN beside one of the other sign or a NaN; but a probability in two terms, one
 // that rounds to zero and the copies that fill a short tile make it inf - inf or 0 * inf. So the values alone decide, taken down far enough
-// that finite ones stay finite. One warp, two rows at a time (more
-// registers here slow the join down), some 240 ns a row; it stops where NaN is all that can come out.
+// that finite ones stay finite. One warp, two rows at a time (four: half the time, but registers that cost the join 1 us of 95 behind a
+// shared prompt), 240 ns a row; it stops where NaN is all that can come out.
 template <typename T, int D>
 __device__ __noinline__ void settle_infinities(const CachedAttnParams& p, int b, int h) {
     constexpr int N = D / 32, AT_ONCE = 2;
@@ -271,8 +274,8 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
     // m is the running maximum less this, so e <= 2^(kGrow + LIFT). fp16 keeps probabilities down to 2^-31 of the largest one that way;
     // the products with bf16 values, which may come near fp32's largest, and their sums stay in range.
     constexpr float LIFT = QUANT ? -kGrow : (std::is_same<T, fp16>::value ? 7.f : -24.f);
-    // P in the operand type is as coarse as the result, except for bf16 results over int8 rows, whose P is fp16. There it takes two
-    // terms, P rounded and what the rounding left, in two products: the tensor cores have the time.
+    // One term of P is as coarse as the result where both have the same type; there P takes two terms, P rounded and what the rounding
+    // left, in two products: the tensor cores have the time. Over int8 rows P is fp16, eight times as fine as a bf16 result: one term.
     constexpr int TERMS = QUANT && std::is_same<T, bf16>::value ? 1 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int sh_sum[4], sh_pos[4];
@@ -790,7 +793,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                     if (last_word) {
                         const float f = ll == 0.f ? 0.f : back / ll;
                         T* dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(row0 + q) * p.o_sh;
-                        float sum = 0.f;
+                        float sum = 0.f;      // finite if all values are
 #pragma unroll
                         for (int i = 0; i < KS; i += 4) {
                             uint32_t w[4];
@@ -798,7 +801,7 @@ __global__ void __launch_bounds__(128, Ring<QUANT, D, NT>::kCtas) cached_attenti
                             for (int j = 0; j < 4; ++j) {
                                 const float2 x = make_float2(acc[nt][i + j][c] * f, acc[nt][i + j][2 + c] * f);
                                 w[j] = Pair<T>::narrow(x);
-                                sum += x.x + x.y;
+                                sum = fmaf(x.x, 0x1p-8f, fmaf(x.y, 0x1p-8f, sum));
                             }
                             *reinterpret_cast<uint4*>(dst + (VW > 4 ? (i >> 2) * 64 + g * 8 : g * KS * 2 + 2 * i)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
@@ -918,12 +921,12 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS) cached_attentio
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * p.o_sh) + lane * (N / 2);
-    float sum = 0.f;
+    float sum = 0.f;                 // finite if all values are
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         const float2 x = make_float2(o[i] * inv, o[i + 1] * inv);
         dst[i / 2] = Pair<T>::narrow(x);
-        sum += x.x + x.y;
+        sum = fmaf(x.x, 0x1p-8f, fmaf(x.y, 0x1p-8f, sum));
     }
     if (__any_sync(0xffffffffu, !(fabsf(sum) < INFINITY)) && l > 0.f) settle_infinities<T, D>(p, b, h);
     if (lane == 0 && p.lse != nullptr) p.lse[b * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;

@@ -408,9 +408,12 @@ bool map_of(const TensorView& t, CUtensorMap* map, int* hfirst) {
 
 // CTAs the blocks are dealt to: a multiple of the pairs (each pair in as many equal ranges), or all SMs (ranges that cross from one pair
 // to the next) where no multiple comes near. All SMs pay only for a large gap, because the power limit lowers the clock with
-// every SM that multiplies: 300 sequences x 64 heads (80 pairs) behind 8192 tokens take 135 us on 148 SMs and 168 on 80, 256 behind
-// 32768 (64 pairs) 340 us on 148 as on 128, 128 behind 16384 (32 pairs) 111 and 100. In microseconds: 2 for a block of a CTA (two 128 x 128 x D products for each of two tiles, or 64 KiB at a 148th of the
-// memory rate), 4 for a segment's start and end, 5 TB/s for the fp32 pieces, written and read back.
+// every SM that multiplies. Whole calls of head dim 128 in us: 300 sequences x 64 heads (80 pairs) behind 8192 tokens 135 on 148
+// SMs, 167 on 80; 256 behind 32768 (64 pairs) 290 on 148 as on 128; 128 behind 16384 (32 pairs) 112 and 100; 64 x 32 heads (8 pairs)
+// behind 8192 53 and 42. The constants are those of head dim 128, in microseconds: 2 for a block of a CTA (two 128 x 128 x D products for
+// each of two tiles, or 64 KiB at a 148th of the memory rate), 4 for a segment's start and end, 5 TB/s for the fp32 pieces, written and
+// read back. At head dim 64, where a block takes less, the same four batches took 113 and 158, 257 and 279 (the choice, 8 % behind
+// the best), 88 either way, 40 and 35; in three more batches of either head dim the choice was the best of all that were tried.
 int plan(int64_t pairs, int64_t blocks, int64_t piece_bytes, int sms) {
     const int64_t total = pairs * blocks;
     auto cost = [&](int64_t ctas) {

@@ -127,8 +127,9 @@ struct Half {
 // neighbouring memory with each access. The rows of a token come
 // in passes of as many rows as the CTA has groups of D / 2H threads, first those of q, then those of k and v; a CTA takes up to
 // kPasses of them and has their loads in flight together. Whether a pass is q or not is the same for the whole CTA, and a thread's
-// angles serve all its rows. Bound by memory: 2 D bytes in per row, 2 D (q) or D + 4 out; 16384 tokens of 32 + 2 x 32 heads of 128 take
-// 153 us, 4.4 TB/s, with the issue slots two thirds busy. kPasses = 3: such a token's three passes in one CTA.
+// angles serve all its rows. Moves 2 D bytes in per row, 2 D (q) or D + 4 out; 16384 tokens of 32 + 2 x 32 heads of 128 take 152 us,
+// 4.4 TB/s. Not at the memory's rate: 5 warps a scheduler (76 registers) keep the issue slots 66 % busy and the ALU 53 %, the
+// rest are waits for fixed latencies and for loads. kPasses = 3: such a token's three passes in one CTA.
 template <typename T, int D, bool INTERLEAVED, int H>
 __global__ void __launch_bounds__(256, 3) rope_quant_append_kernel(const AppendParams p) {
     constexpr int LANES = D / (2 * H), ROWS = 256 / LANES;
@@ -257,7 +258,7 @@ struct DequantParams {
 
 // D / 16 threads take a row, 8 values of each half: a CTA takes 256 / (D / 16) heads of kTokens tokens, of k and of v, with all loads
 // in flight. A code becomes fp32 as the low byte of 2^23 + 128 + code, exactly, and then one product is rounded.
-// Bound by memory: D + 4 bytes in, 2 D out; 16384 tokens of 2 x 32 heads of 128 take 65 us, 6.2 TB/s.
+// Bound by memory: D + 4 bytes in, 2 D out; 16384 tokens of 2 x 32 heads of 128 take 64 us, 6.3 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
     constexpr int LANES = D / 16, ROWS = 256 / LANES;

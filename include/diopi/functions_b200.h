@@ -113,10 +113,13 @@ DIOPI_API diopiError_t diopiB200RopeAppendKV(diopiContextHandle_t ctx, diopiTens
  * diopiB200CachedAttention  out [B, Hq, D] = softmax(scale * q K^T) V over the first lengths[b] slots (clamped to [0, L]) of sequence
  *                      b's cache; Hq / Hkv query heads share a key head. k_scale / v_scale NULL: k_cache / v_cache
  *                      hold q's dtype (pitches multiples of 8 elements). An empty sequence gives zeros and a
- *                      softmax_lse of -inf. softmax_lse: optional float32 [B, Hq], the log of the softmax denominator.
+ *                      softmax_lse of -inf. softmax_lse: optional float32 [B, Hq], the log of the softmax denominator. Sums are fp32. A
+ *                      probability enters the product with the values rounded to 2^-11 of itself (bfloat16 results over int8 rows) or to
+ *                      2^-16 and finer; one below 2^-31 of its row's largest may be lost (over int8 rows each times its value scale;
+ *                      over bfloat16 rows far below that). An infinity among the visible values gives that infinity.
  * diopiB200SharedPrefixAttention  the same over the rows of a prompt that all sequences share, prefix_k / prefix_v [P, Hkv, D] in q's
  *                      dtype (positive pitches that are multiples of 8, one a multiple of the other), followed by the sequence's own lengths[b] slots. The
- *                      prompt is stored once and read once for the batch.
+ *                      prompt is stored once and read once for the batch. A probability of its rows is rounded to q's dtype, in one term.
  * out must not overlap an input. The attention calls take workspace through diopiRequireBuffer; a graph that captured one needs
  * that workspace for its replays, so its context keeps it (no release, no other use of the context) while the graph lives. */
 DIOPI_API diopiError_t diopiB200RopeQuantAppendKV(diopiContextHandle_t ctx, diopiTensorHandle_t q_out, diopiConstTensorHandle_t qkv,
