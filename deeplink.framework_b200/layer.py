@@ -617,8 +617,8 @@ class DecoderLayer:
         try:
             out = self.decode_cached(x, cache, positions, lengths, prefix, ctx)
         finally:
-            graph = devapis.graphEndCapture(ctx.stream)
             keep, self._keep = self._keep, None
+            graph = devapis.graphEndCapture(ctx.stream)
 
         def replay(_keep=keep):
             devapis.graphLaunch(graph, ctx.stream)

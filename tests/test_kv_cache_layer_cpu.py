@@ -53,3 +53,27 @@ def test_tables_hold_the_positions_behind_the_prompt(lay):
             assert t.is_contiguous() and t.data_ptr() % 16 == 0
         kept.append((cos, cos.clone()))
     assert all(torch.equal(a, b) for a, b in kept)   # a captured step goes on reading the table it was captured with
+
+
+def test_a_capture_that_fails_leaves_the_layer_as_it_was(lay, monkeypatch):
+    """An error inside the step ends the capture, which may fail in turn; later calls must not go on keeping their temporaries."""
+    from dipu_b200 import layer as L
+
+    class StepError(Exception):
+        pass
+
+    def step(*args):
+        raise StepError
+
+    ended = []
+
+    def end(stream):
+        ended.append(stream)
+        raise RuntimeError("the capture was invalidated")
+
+    monkeypatch.setattr(L.devapis, "graphBeginCapture", lambda stream: None)
+    monkeypatch.setattr(L.devapis, "graphEndCapture", end)
+    monkeypatch.setattr(lay, "decode_cached", step)
+    with pytest.raises((StepError, RuntimeError)):
+        lay.capture_decode_cached(None, _Cache, None, None, stream=0)
+    assert ended and lay._keep is None
