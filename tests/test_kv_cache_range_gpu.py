@@ -140,9 +140,34 @@ KINDS = [(True, BF), (True, FP), (False, BF), (False, FP)]
 @pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 128), (14, 2, 64), (16, 1, 128), (24, 1, 128)])
 @pytest.mark.parametrize("quant,dtype", KINDS)
 def test_probabilities_in_two_terms(pkg, ctx, quant, dtype, Hq, Hkv, D):
-    """Results that are small beside sum p |v| would show a probability of one term. Whole segments and pieces."""
+    """Whole segments and pieces, held to the bound of two terms."""
     for L, lengths in ((300, [300, 0, 1, 77]), (900, [900, 640, 17, 65])):
         _hold(pkg, ctx, _randn((4, Hq, D), 1, dtype).to(DEV), _cache(quant, dtype, 4, Hkv, L, D), lengths, D ** -0.5)
+
+
+def _two_groups(quant, dtype, B, n):
+    """Sequence b: even keys have score 0, odd ones 8 t = -(b + 1) / 16; the values of the two groups cancel, and all keys of a group
+    have the same probability, so that its rounding does not average out. q, cache, t."""
+    D = 64
+    q = torch.ones((B, 1, D), dtype=dtype, device=DEV)
+    odd = torch.arange(n, device=DEV) % 2 == 1
+    t = -(torch.arange(B, device=DEV) + 1) / 128.0
+    if quant:
+        k, v = (torch.full((B, 1, n, D), 64, dtype=torch.int8, device=DEV) for _ in range(2))
+        v[:, :, odd] = -37
+        ks = torch.where(odd, t[:, None, None] / 64, torch.zeros((), device=DEV))
+        vs = torch.where(odd, 0.01 * 64 / 37 * torch.exp(-8 * t)[:, None, None], torch.full((), 0.01, device=DEV))
+        return q, [k, ks, v, vs], t
+    k = torch.where(odd[None, None, :, None], t[:, None, None, None], torch.zeros((), device=DEV)).expand(B, 1, n, D)
+    v = torch.where(odd[None, None, :, None], -torch.exp(-8 * t)[:, None, None, None], torch.ones((), device=DEV)).expand(B, 1, n, D)
+    return q, [k.to(dtype).contiguous(), None, v.to(dtype).contiguous(), None], t
+
+
+@pytest.mark.parametrize("quant,dtype", [(True, FP), (False, BF), (False, FP)])
+@pytest.mark.parametrize("n", [256, 600])
+def test_one_term_would_show(pkg, ctx, quant, dtype, n):
+    q, cache, _ = _two_groups(quant, dtype, 12, n)
+    _hold(pkg, ctx, q, cache, [n] * 12, 0.125)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
